@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define ME_ABI_VERSION 24
+#define ME_ABI_VERSION 25
 #define ME_DEC_PART_REC(dh) ((dh) + 4)      /* floats per attention partial of the decode step (me_dec_attn) */
 #define ME_SUMSQ_WS_BYTES 1040   /* me_sumsq workspace: ticket counter + 256 block sums + padding */
 
@@ -169,7 +169,8 @@ enum {
     ME_WS_EMBED_BWD = 6,     /* me_embed_bwd frequent-token list: 1024 bytes, zero before the first use */
     ME_WS_SUMSQ = 7,         /* me_sumsq ordered block sums: ME_SUMSQ_WS_BYTES, zero before the first use */
     ME_WS_RELU_MASK = 8,     /* me_gemm_nt_relu_mask sign mask: (M, N, K) = the product's; 0 = shape / dtype not served, use the gate */
-    ME_WS_DEC_TOKEN = 9      /* me_dec_token exchange records: (M, N, K) = (Mr, d_inner, d); zero before the first use */
+    ME_WS_DEC_TOKEN = 9,     /* me_dec_token exchange records: (M, N, K) = (Mr, d_inner, d); zero before the first use */
+    ME_WS_KVQ_ATTN = 10      /* me_kvq_attn partial records: (M, N, K) = (B * H, nsplit, dh) */
 };
 size_t me_workspace_bytes(int op, int M, int N, int K, int dtype);
 
@@ -441,6 +442,46 @@ int me_dec_token(const int64_t* tokens, const float* cond, const float* emb, con
                  int M, int Mc, int t, const int32_t* t_dev, float eps, int blocks, int dtype, void* stream);
 /* Largest number of co-resident blocks the device gives me_dec_token for this dtype / dh (0: shape not served). */
 int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
+
+/* ---- quantised key / value cache ------------------------------------------------------------------------------------
+ * The caches of the decode step (generate.py:92-122 made incremental) in 4 or 8 bits: a row (one token, one head) of dh
+ * values is held as dh codes and one bfloat16 scale,
+ *   scale = amax / top, top = 6 (4 bits: e2m1) or 448 (8 bits: e4m3); f32 quotient cut (not rounded) to bfloat16,
+ *   code  = x / scale to the nearest value of the code's type, ties to the even code, larger ones to the largest;
+ * a row with amax < 2^-96 is held as zeros (scale 0), a row with an infinity or a NaN reads back as NaN (scale NaN, codes 0).
+ * 32 tokens form a block; `blocks` of them per (sequence, head) are the cache's room:
+ *   kcodes / vcodes : uint8 [B][H][blocks][32 * dh * bits / 8], 16-byte aligned, ZERO before the first use
+ *   kscale / vscale : bfloat16 [B][H][blocks * 32]
+ * Order of the codes inside a block (position p counts codes; 4 bits: byte p / 2, low nibble first):
+ *   K, 4 bits: p = (group * 16 + token % 16) * 32 + i;  dh 64: group = 2 (token / 16) + d / 32, i = d % 32;  dh 32: group = token / 16,
+ *      i = d;  dh 48: d < 32: group = 2 (token / 16), i = d;  else group = 1, i = 16 (token / 16) + d - 32
+ *   V, 4 bits: p = d * 32 + token
+ *   8 bits: K: p = (i / 16) * 16 dh + (group * 16 + token % 16) * 16 + i % 16;  V: p = (token / 16) * 16 dh + d * 16 + token % 16
+ * dh in {32, 48, 64}.  Positions: t for all sequences, or t_dev (device int32, may be NULL) = one value for all (ld_t = 0) or one
+ * per sequence (ld_t = 1); a device position is read by the kernels and never checked by the host: tokens that have no place in the
+ * cache are left out.
+ *
+ * me_kvq_write: rows [B][n][H][dh] of T (strides: six element counts {k: sequence, token, head, v: sequence, token, head}, dh
+ *   contiguous; a HOST array read during the call) to positions t .. t + n - 1.  lens (device int32 [B] or NULL): only the first
+ *   lens[b] rows of sequence b.  Codes and scales of every other token stay as they were.  n <= 32 * blocks.
+ * me_kvq_read: rows at positions t .. t + n - 1 as T(code * scale), one rounding; rows from lens[b] on, and those behind the
+ *   cache's end, are written as zeros.
+ * me_kvq_attn: one query per (sequence, head), q / out: T [B][H][dh] with strides ldq_* / ldo_* (elements):
+ *     out = sum_j softmax_j( (q.k_j + q.E[M-1-(t-j)]) / sqrt(dh) ) v_j   over keys j = 0 .. t that key_pad leaves (music_multi.py:211-235)
+ *   E (T [M][dh] natural layout, 16-byte aligned; NULL: no relative term) needs M >= 32 * blocks.  key_pad: uint8 [B][ld_pad] or NULL,
+ *   1 = masked; keys from ld_pad on are not masked.  A masked row's codes and scale are never used, whatever they hold.  No
+ *   key left (t = -1, or all masked): zeros.  nsplit in 1 .. 64 key ranges (me_kvq_splits gives a good number); with nsplit > 1
+ *   `part` (me_workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh, dtype) bytes, 16-byte aligned, uninitialised, private to the
+ *   call until it has run) holds the ranges' records and a second launch joins them in ascending order.  out = NULL: the records are the
+ *   result, as me_dec_attn leaves them (nsplit <= 8: me_dec_proj_resid joins them; it takes a row without keys for NaN). */
+int me_kvq_write(const void* k, const void* v, const int64_t* strides, void* kcodes, void* kscale, void* vcodes, void* vscale, int B, int n,
+                 int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, const int32_t* lens, int dtype, void* stream);
+int me_kvq_read(const void* kcodes, const void* kscale, const void* vcodes, const void* vscale, void* k, void* v, const int64_t* strides, int B,
+                int n, int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, const int32_t* lens, int dtype, void* stream);
+int me_kvq_splits(int B, int H, int tokens);
+int me_kvq_attn(const void* q, int64_t ldq_b, int64_t ldq_h, const void* kcodes, const void* kscale, const void* vcodes, const void* vscale,
+                const void* E, int M, const uint8_t* key_pad, int ld_pad, void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes,
+                int nsplit, int B, int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, int dtype, void* stream);
 
 /* Greedy pick for generate(top_k=1): logits f32 [B, ld]; NaN -> 0, ids in
  * special[0..n_special) -> -inf, argmax -> out_ids[B] (generate.py:122-136,166-183). */

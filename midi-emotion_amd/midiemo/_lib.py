@@ -12,9 +12,9 @@ LIB_PATH = os.environ.get("MIDIEMO_LIB") or os.path.join(HERE, "libmidiemo_hip.s
 ME_F32, ME_BF16, ME_F16 = 0, 1, 2
 ME_COND_NONE, ME_COND_CONCAT, ME_COND_TOKEN = 0, 1, 2
 ME_EPI_RELU, ME_EPI_OUT_F32, ME_EPI_RELU_BWD = 1, 2, 4
-ME_WS_GEMM_TN, ME_WS_RGA_PT, ME_WS_RGA_DGT, ME_WS_RGA_MT, ME_WS_GEMM_TN_GROUP, ME_WS_EMBED_BWD, ME_WS_SUMSQ, ME_WS_RELU_MASK, ME_WS_DEC_TOKEN = 1, 2, 3, 4, 5, 6, 7, 8, 9
+ME_WS_GEMM_TN, ME_WS_RGA_PT, ME_WS_RGA_DGT, ME_WS_RGA_MT, ME_WS_GEMM_TN_GROUP, ME_WS_EMBED_BWD, ME_WS_SUMSQ, ME_WS_RELU_MASK, ME_WS_DEC_TOKEN, ME_WS_KVQ_ATTN = 1, 2, 3, 4, 5, 6, 7, 8, 9, 10
 ME_TN_MAX_GROUP = 5
-ABI_VERSION = 24
+ABI_VERSION = 25
 ME_LO8 = 0x100             # OR-ed into the dtype of me_resid_ln_fwd / me_embed_fwd: 8-bit low halves of the residual stream
 ME_DEC_MAX_LAYERS, ME_DEC_TOKEN_ROWS = 16, 4
 # words of the loss-scaler state (me_scaler_step; enum ME_SCALER_* of include/midiemo.h)
@@ -59,6 +59,10 @@ SIGNATURES = {
     "me_dec_ln_proj": [_p, _p, _p, _f, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
     "me_dec_token": [_p, _p, _p, _p, _p, _p, _i, _p, _i, _p, _i, _p, _i, _p, _i, _p, ctypes.c_size_t, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _f, _i, _i, _p],
     "me_dec_token_blocks": [_i, _i, _i, _i],
+    "me_kvq_write": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _i, _p],
+    "me_kvq_read": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _i, _p],
+    "me_kvq_splits": [_i, _i, _i],
+    "me_kvq_attn": [_p, _i64, _i64, _p, _p, _p, _p, _p, _i, _p, _i, _p, _i64, _i64, _p, ctypes.c_size_t, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _p],
     "me_greedy_pick": [_p, _i, _i, _p, _i, _p, _i, _p],
     "me_sample_topk_topp": [_p, _i, _i, _p, _i, _p, _i, _f, _p, _p, _p, _p, _p, _i, _p],
     "me_sample_step": [_p, _i, _i, _p, _i, _p, _p, _p, _f, _f, _f, _i, _f, _p, _i, _p, _i, _p, _p, _i, _p],

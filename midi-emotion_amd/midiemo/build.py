@@ -9,12 +9,19 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 INCLUDE = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include")
 LIB = os.path.join(HERE, "libmidiemo_hip.so")
-SOURCES = ["me_gemm.hip", "me_elem.hip", "me_attn.hip", "me_attn64.hip", "me_decode.hip", "me_decode_token.hip"]
+SOURCES = ["me_gemm.hip", "me_elem.hip", "me_attn.hip", "me_attn64.hip", "me_decode.hip", "me_decode_token.hip", "me_kvq.hip"]
 # -amdgpu-mfma-vgpr-form: keep MFMA accumulators in VGPRs.  Without it hipcc parks the accumulators of loops whose
 # MFMAs sit under a wave-uniform branch in AGPRs and copies all of them (v_accvgpr_read/write) around every
 # iteration: 128 of ~250 VALU instructions per step in rga_bwd_kv, 96 of ~230 in rga_bwd_e.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-value",
          "-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+
+# No v_pk_{add,mul,fma}_f32: the compiler forms them from ordinary scalar code, and some of their forms have given wrong results on this
+# part now and then, without an error (the host pass warns that it does not know the feature).  The files of FIXED_ROUNDING are compiled
+# as they always were: without the feature their sums are contracted in another way, and tests that pin their roundings fail
+# (test_dec_ln_proj and test_resid_ln_fwd_bwd in f16, each by one rounding step).
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FIXED_ROUNDING = ("me_gemm.hip", "me_elem.hip", "me_attn.hip", "me_attn64.hip", "me_decode.hip", "me_decode_token.hip")
 
 
 def _hipcc():
@@ -41,7 +48,7 @@ def build(force=False, verbose=False):
         obj = os.path.join(CSRC, s.replace(".hip", ".o"))
         objs.append(obj)
         if force or _stale(obj, [src] + common):
-            cmd = [hipcc] + FLAGS + ["-c", src, "-o", obj]
+            cmd = [hipcc] + FLAGS + ([] if s in FIXED_ROUNDING else NO_PACKED) + ["-c", src, "-o", obj]
             if verbose:
                 print(" ".join(cmd))
             procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))

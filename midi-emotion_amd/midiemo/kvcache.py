@@ -1,0 +1,132 @@
+"""Key / value cache in 4 or 8 bits (csrc/me_kvq.hip): rows are quantised as they are written, attended to as they lie, and
+can be read back.
+
+A row (one token, one head) of head_dim values is held as 4-bit e2m1 or 8-bit e4m3 codes and one bfloat16 scale (amax / 6 or amax / 448,
+cut to bfloat16): 34 or 66 bytes at head_dim 64 against 128 in bf16.  The codes lie in the order in which the matrix instructions take
+them (include/midiemo.h describes it), 32 tokens to a block.  The decode step this serves: generate.py:92-122 of the
+reference, made incremental; the attention is music_multi.py:211-235 for one query row."""
+import torch
+
+from . import ops
+
+HEAD_DIMS = (32, 48, 64)
+BLOCK = 32
+
+
+def _need(ok, what):
+    if not ok:
+        raise RuntimeError("kv cache: " + what)
+
+
+class QuantKVCache:
+    """Cache of `batch` sequences, `heads` heads, at least `max_len` tokens (rounded up to blocks of 32).
+
+    Positions (`pos` below) are a whole number, or an int32 device tensor of one value or one per sequence; those are read on the
+    device (so a captured step can advance them) and rows without a place in the cache are then left out instead of
+    refused.  Calls only enqueue work on the current stream of the cache's device."""
+
+    def __init__(self, batch, heads, max_len, head_dim, bits=4, device="cuda"):
+        _need(batch > 0 and heads > 0 and max_len > 0, "batch, heads and max_len must be positive")
+        _need(head_dim in HEAD_DIMS and bits in (4, 8), "head_dim must be 32, 48 or 64 and bits 4 or 8 (got %r, %r)" % (head_dim, bits))
+        blocks = -(-int(max_len) // BLOCK)
+        z = lambda *s, dtype: torch.zeros(*s, dtype=dtype, device=device)
+        size = BLOCK * head_dim * bits // 8
+        self._set(z(batch, heads, blocks, size, dtype=torch.uint8), z(batch, heads, blocks * BLOCK, dtype=torch.bfloat16),
+                  z(batch, heads, blocks, size, dtype=torch.uint8), z(batch, heads, blocks * BLOCK, dtype=torch.bfloat16), head_dim, bits)
+
+    @classmethod
+    def wrap(cls, k, k_scale, v, v_scale, head_dim, bits):
+        """A cache over existing tensors: codes uint8 [B, H, blocks, 32 * head_dim * bits / 8], scales bfloat16 [B, H, blocks * 32]."""
+        self = cls.__new__(cls)
+        _need(head_dim in HEAD_DIMS and bits in (4, 8), "head_dim must be 32, 48 or 64 and bits 4 or 8 (got %r, %r)" % (head_dim, bits))
+        _need(k.dim() == 4 and all(x > 0 for x in k.shape) and k.shape[3] == BLOCK * head_dim * bits // 8, "codes must be [B, H, blocks, %d], got %s" % (BLOCK * head_dim * bits // 8, tuple(k.shape)))
+        for t, shape, dtype in ((k, k.shape, torch.uint8), (v, k.shape, torch.uint8), (k_scale, (*k.shape[:2], k.shape[2] * BLOCK), torch.bfloat16),
+                                (v_scale, (*k.shape[:2], k.shape[2] * BLOCK), torch.bfloat16)):
+            _need(t.shape == shape and t.dtype == dtype and t.is_contiguous() and t.device == k.device, "codes and scales must be contiguous tensors of matching shapes and types on one device")
+        self._set(k, k_scale, v, v_scale, head_dim, bits)
+        return self
+
+    def _set(self, k, k_scale, v, v_scale, head_dim, bits):
+        self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
+        self.batch, self.heads, self.head_dim, self.bits = k.shape[0], k.shape[1], head_dim, bits
+        self.max_len = k.shape[2] * BLOCK
+        self.device = k.device
+        self.nbytes = 2 * (k.numel() + 2 * k_scale.numel())
+
+    # -------------------------------------------------------------- checks
+    def _here(self, *tensors):
+        for t in tensors:
+            _need(t is None or t.device == self.device, "a tensor is on %s, the cache on %s" % (None if t is None else t.device, self.device))
+
+    def _pos(self, pos, n):
+        if isinstance(pos, torch.Tensor):
+            _need(pos.dtype == torch.int32 and pos.is_contiguous() and pos.numel() in (1, self.batch), "a position tensor must be int32 with 1 or %d values" % self.batch)
+            self._here(pos)
+        else:
+            _need(0 <= int(pos) and int(pos) + n <= self.max_len, "positions %d..%d do not fit %d tokens" % (int(pos), int(pos) + n - 1, self.max_len))
+
+    def _rows(self, k, v, pos, lens):
+        for x in (k, v):
+            _need(x.dim() == 4 and x.shape == k.shape and x.shape[0] == self.batch and x.shape[2:] == (self.heads, self.head_dim) and x.dtype == k.dtype and
+                  (x.stride(3) == 1 or x.numel() == 0), "rows must be [%d, n, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
+        _need(k.shape[1] <= self.max_len, "%d rows do not fit %d tokens" % (k.shape[1], self.max_len))
+        _need(lens is None or (lens.dtype == torch.int32 and lens.shape == (self.batch,) and lens.is_contiguous()), "lens must be int32 [%d]" % self.batch)
+        self._here(k, v, lens)
+        self._pos(pos, k.shape[1])
+
+    def _on(self):
+        _need(self.device.type == "cuda", "it is on %s -- there is no CPU path" % self.device)
+        return torch.cuda.device(self.device)
+
+    # -------------------------------------------------------------- calls
+    def write(self, k, v, pos, lens=None):
+        """Quantise k, v [B, n, H, head_dim] (float32, bfloat16 or float16; any strides, last dimension contiguous) into positions pos .. pos + n - 1;
+        with lens (int32 [B]) only the first lens[b] rows of sequence b.  Everything else in the cache stays as it was."""
+        self._rows(k, v, pos, lens)
+        if k.shape[1] == 0:
+            return
+        with self._on():
+            ops.kvq_write(k, v, self.k, self.k_scale, self.v, self.v_scale, self.bits, pos, lens)
+
+    def read(self, pos, n, dtype=torch.float32, lens=None):
+        """The rows at positions pos .. pos + n - 1 as (k, v) [B, n, H, head_dim] of `dtype`; rows from lens[b] on are zeros."""
+        k = torch.empty(self.batch, int(n), self.heads, self.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        self._rows(k, v, pos, lens)
+        with self._on():
+            if k.shape[1] > 0:
+                ops.kvq_read(self.k, self.k_scale, self.v, self.v_scale, k, v, self.bits, pos, lens)
+        return k, v
+
+    def attend(self, q, pos, rel=None, key_pad=None, out=None, nsplit=0):
+        """softmax((q.k_j + q.rel[M-1-(pos-j)]) / sqrt(head_dim)) v over the cached keys j = 0 .. pos (pos = -1: none).
+
+        q [B, H, head_dim]; rel [M, head_dim] of q's type with M >= max_len (the model's relative table) or None; key_pad uint8 / bool
+        [B, n], 1 = masked key.  A row without a key gives zeros.  nsplit: key ranges that run side by side (0: chosen from the sizes)."""
+        _need(q.dim() == 3 and q.shape == (self.batch, self.heads, self.head_dim) and q.stride(2) == 1, "q must be [%d, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(q.shape)))
+        if rel is not None:
+            _need(rel.dim() == 2 and rel.shape[1] == self.head_dim and rel.shape[0] >= self.max_len and rel.is_contiguous() and rel.dtype == q.dtype,
+                  "rel must be a contiguous [>= %d, %d] table of q's type" % (self.max_len, self.head_dim))
+        if key_pad is not None:
+            if key_pad.dtype == torch.bool:
+                key_pad = key_pad.view(torch.uint8)
+            _need(key_pad.dtype == torch.uint8 and key_pad.dim() == 2 and key_pad.shape[0] == self.batch and key_pad.is_contiguous(),
+                  "key_pad must be contiguous uint8 or bool [%d, n]" % self.batch)
+            _need(isinstance(pos, torch.Tensor) or key_pad.shape[1] > int(pos), "key_pad is narrower than the %d keys" % (0 if isinstance(pos, torch.Tensor) else int(pos) + 1))
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1 and all(s != 0 or x == 1 for s, x in zip(out.stride(), out.shape)), "out must match q")
+        self._here(q, rel, key_pad, out)
+        if isinstance(pos, torch.Tensor):
+            self._pos(pos, 1)
+            tokens = self.max_len
+        else:
+            _need(-1 <= int(pos) < self.max_len, "position %d does not fit %d tokens" % (int(pos), self.max_len))
+            tokens = max(int(pos) + 1, 1)
+        _need(0 <= nsplit <= 64, "nsplit must be 0..64")
+        with self._on():
+            ns = nsplit or ops.kvq_splits(self.batch, self.heads, tokens)
+            # the records of this call: from the caching allocator, so calls on two streams or in two captured graphs never share them
+            part = torch.empty(self.batch * self.heads * ns * (self.head_dim + 4), dtype=torch.float32, device=self.device) if ns > 1 else None
+            ops.kvq_attn(q, self.k, self.k_scale, self.v, self.v_scale, out, self.bits, pos, rel, key_pad, part, ns)
+        return out

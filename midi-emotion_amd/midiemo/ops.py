@@ -10,7 +10,7 @@ import torch
 from . import _lib
 from ._lib import (ME_BF16, ME_F16, ME_COND_CONCAT, ME_COND_NONE, ME_COND_TOKEN, ME_EPI_OUT_F32, ME_EPI_RELU,
                    ME_EPI_RELU_BWD, ME_F32, ME_TN_MAX_GROUP, ME_WS_EMBED_BWD, ME_WS_SUMSQ, ME_WS_GEMM_TN, ME_WS_GEMM_TN_GROUP, ME_WS_RGA_DGT, ME_WS_RGA_MT,
-                   ME_WS_RGA_PT, ME_WS_RELU_MASK, ME_WS_DEC_TOKEN, check)
+                   ME_WS_RGA_PT, ME_WS_RELU_MASK, ME_WS_DEC_TOKEN, ME_WS_KVQ_ATTN, check)
 
 DTYPE_CODE = {torch.float32: ME_F32, torch.bfloat16: ME_BF16, torch.float16: ME_F16}
 
@@ -369,6 +369,50 @@ def dec_token(tokens, cond, emb, cw, cb, pe, d_cond, table, n_layer, Wf, bf, V, 
                              int(nsplit), int(Mr), int(d), int(d_inner), int(H), int(dh), int(M), int(Mc), int(t), _ptr(t_dev), float(eps),
                              int(blocks), _code(dtype), _stream()), "me_dec_token")
 
+
+
+def _pos_args(pos):
+    """(t, t_dev, ld_t) of a position: a whole number, or an int32 device tensor of one value or one per sequence."""
+    if isinstance(pos, torch.Tensor):
+        return 0, _ptr(pos), 1 if pos.numel() > 1 else 0
+    return int(pos), None, 0
+
+
+_I64x6 = ctypes.c_int64 * 6
+
+
+def kvq_write(k, v, kcodes, kscale, vcodes, vscale, bits, pos, lens=None):
+    """quantise the rows k, v [B, n, H, dh] (any strides, dh contiguous) into the cache at positions pos .. (me_kvq_write)."""
+    B, n, H, dh = k.shape
+    t, t_dev, ld_t = _pos_args(pos)
+    check(lib().me_kvq_write(_ptr(k), _ptr(v), _I64x6(*k.stride()[:3], *v.stride()[:3]), _ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale),
+                             B, n, H, dh, kcodes.shape[2], int(bits), t, t_dev, ld_t, _ptr(lens), _code(k.dtype), _stream()), "me_kvq_write")
+
+
+def kvq_read(kcodes, kscale, vcodes, vscale, k, v, bits, pos, lens=None):
+    """the rows at positions pos .. pos + n - 1 into k, v [B, n, H, dh] (me_kvq_read); rows from lens[b] on become zeros."""
+    B, n, H, dh = k.shape
+    t, t_dev, ld_t = _pos_args(pos)
+    check(lib().me_kvq_read(_ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale), _ptr(k), _ptr(v), _I64x6(*k.stride()[:3], *v.stride()[:3]),
+                            B, n, H, dh, kcodes.shape[2], int(bits), t, t_dev, ld_t, _ptr(lens), _code(k.dtype), _stream()), "me_kvq_read")
+
+
+def kvq_splits(B, H, tokens):
+    """key ranges me_kvq_attn should cut a cache of that many tokens into (1 .. 64)"""
+    return int(lib().me_kvq_splits(int(B), int(H), int(tokens)))
+
+
+def kvq_attn(q, kcodes, kscale, vcodes, vscale, out, bits, pos, E=None, key_pad=None, part=None, nsplit=1):
+    """attention of one query per (sequence, head), q / out [B, H, dh], against the cached keys 0 .. pos (me_kvq_attn).
+    part: uninitialised f32 buffer of workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh) bytes where nsplit > 1; out = None
+    leaves the partial records in it (the form me_dec_proj_resid reads)."""
+    B, H, dh = q.shape
+    t, t_dev, ld_t = _pos_args(pos)
+    check(lib().me_kvq_attn(_ptr(q), q.stride(0), q.stride(1), _ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale), _ptr(E),
+                            E.shape[0] if E is not None else 0, _ptr(key_pad), key_pad.stride(0) if key_pad is not None else 0, _ptr(out),
+                            out.stride(0) if out is not None else 0, out.stride(1) if out is not None else 0, _ptr(part),
+                            part.numel() * part.element_size() if part is not None else 0, int(nsplit), B, H, dh, kcodes.shape[2], int(bits), t,
+                            t_dev, ld_t, _code(q.dtype), _stream()), "me_kvq_attn")
 
 
 def sample_topk_topp(logits, V, special, temp, top_k, top_p, u, out_ids, n_choices=None, dbg_p=None, dbg_i=None):
