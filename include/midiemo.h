@@ -510,6 +510,26 @@ int me_sample_step(const float* logits, int ld, int V, const int32_t* special, i
                    int top_k, float top_p, const float* u_table, int u_ld, const int32_t* pos, int pos0, int64_t* out_ids,
                    int32_t* n_choices, int B, void* stream);
 
+/* Sampling with min-p and for wide vocabularies (V <= ME_SAMPLE_MAX_VOCAB), one launch for the whole batch: the rules of
+ * me_sample_topk_topp with min-p behind them and the arithmetic in 64 bits.  NaN -> 0, ids in special[] -> -inf; entries in the order
+ * (logit descending, index ascending); weight w = exp((x - max x) / temp[b]); kept are the entries that pass all of
+ *   top_k  (> 0): the first top_k entries;
+ *   top_p  (0 < top_p < 1): the first entry, and those whose cumulative weight (their own included) is at most top_p of the sum over
+ *          what top_k keeps;
+ *   min_p  (0 <= min_p <= 1): w >= min_p, min_p times the weight of the most likely entry;   and w > 0 in 64 bits.
+ * out_ids[b] = the first kept entry at which the cumulative weight exceeds u[b] times the sum of the kept ones (u in [0, 1); a u of 1 and
+ * more: the last one that has a weight); n_choices[b] (may be NULL) = number of kept entries.  A row with every logit -inf: id 0, 0 choices;
+ * several +inf share the weight.  Cumulative weights are exact sums of weights rounded to 2^-45, so results do not depend on scheduling.
+ * temp[b] must be positive and finite.
+ * me_sample_minp_step is the same for a step of a device-resident loop (arguments of me_sample_step). */
+#define ME_SAMPLE_MAX_VOCAB (1 << 18)
+int me_sample_minp(const float* logits, int ld, int V, const int32_t* special, int n_special, const float* temp, int top_k, float top_p,
+                   float min_p, const float* u, int64_t* out_ids, int32_t* n_choices, int B, void* stream);
+int me_sample_minp_step(const float* logits, int ld, int V, const int32_t* special, int n_special, const int64_t* prev_tok,
+                        const uint8_t* is_timeshift, float* repeat_counts, float temp_note, float temp_rest, float penalty_coeff, int top_k,
+                        float top_p, float min_p, const float* u_table, int u_ld, const int32_t* pos, int pos0, int64_t* out_ids,
+                        int32_t* n_choices, int B, void* stream);
+
 /* Device-side decode bookkeeping: history[b][*pos] = tok[b] (int64 [B][ld_hist]); *pos += 1.
  * With me_embed_fwd(pos_dev) and the t_dev arguments of me_dec_* a greedy decode step has no host-side state
  * (the token loop of generate.py:99-189 for top_k = 1) and can be captured once and replayed. */

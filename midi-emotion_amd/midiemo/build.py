@@ -9,7 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 INCLUDE = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include")
 LIB = os.path.join(HERE, "libmidiemo_hip.so")
-SOURCES = ["me_gemm.hip", "me_elem.hip", "me_attn.hip", "me_attn64.hip", "me_decode.hip", "me_decode_token.hip", "me_kvq.hip"]
+SOURCES = ["me_gemm.hip", "me_elem.hip", "me_attn.hip", "me_attn64.hip", "me_decode.hip", "me_decode_token.hip", "me_kvq.hip", "me_sample.hip"]
 # -amdgpu-mfma-vgpr-form: keep MFMA accumulators in VGPRs.  Without it hipcc parks the accumulators of loops whose
 # MFMAs sit under a wave-uniform branch in AGPRs and copies all of them (v_accvgpr_read/write) around every
 # iteration: 128 of ~250 VALU instructions per step in rga_bwd_kv, 96 of ~230 in rga_bwd_e.
