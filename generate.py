@@ -61,10 +61,12 @@ def generate(model, maps, device, out_dir, conditioning, short_filename=False,
              gen_len=2048, temperatures=[1.2, 1.2], top_k=-1,
              top_p=0.7, debug=False, varying_condition=None, seed=-1,
              verbose=False, primers=[["<START>"]], min_n_instruments=2,
-             use_cache=True, return_ids=False, device_loop=True, use_window_graph=True):
+             use_cache=True, return_ids=False, device_loop=True, use_window_graph=True, min_p=0.0, kv_bits=None):
     """Reference signature (generate.py:20-26) + `use_cache`, `return_ids`, `device_loop` (sampling loop replayed on
     the device as one HIP graph per token while the KV cache is valid; False = one Python iteration per token) and
     `use_window_graph` (once the window slides, its full forward is replayed as one HIP graph per token).
+    `min_p` > 0 drops tokens less likely than min_p times the most likely one (after top-k and the nucleus); `kv_bits` = 4 or 8 holds
+    the KV cache quantised.
     `amp` is accepted for compatibility; the engine's precision is model.compute_dtype."""
     if not debug:
         os.makedirs(out_dir, exist_ok=True)
@@ -122,12 +124,16 @@ def generate(model, maps, device, out_dir, conditioning, short_filename=False,
     repeat_counts = torch.zeros(batch_size, device=device)
     temp_note, temp_rest = float(temperatures[0]), float(temperatures[1])
     V = model.vocab_size
-    if V > 4096 and top_k != 1:
-        # the device sampling tail (me_sample_topk_topp / me_sample_step) sorts one row of (value, id) pairs in LDS: 1024,
-        # 2048 or 4096 wide (the reference's vocabularies have 1007 / 1017 / 1018 symbols).  There is no second, non-HIP
-        # sampling path in this build; greedy decoding (--topk 1) has no limit.
-        raise NotImplementedError("sampled generation supports vocabularies of at most 4096 symbols (got %d); "
-                                  "use top_k=1 (greedy) or add a wider instantiation of sample_kernel" % V)
+    max_vocab = ops._lib.ME_SAMPLE_MAX_VOCAB
+    if V > max_vocab and top_k != 1:
+        # rows of up to 4096 symbols are sorted in LDS (me_sample_topk_topp / me_sample_step; the reference's vocabularies have 1007 /
+        # 1017 / 1018), wider ones and min-p go through me_sample_minp.  There is no second, non-HIP sampling path in this
+        # build; greedy decoding (--topk 1) has no limit.
+        raise NotImplementedError("sampled generation supports vocabularies of at most %d symbols (got %d); use top_k=1 (greedy)" % (max_vocab, V))
+    if not 0 <= min_p <= 1:
+        raise ValueError("min_p must lie in [0, 1] (got %r)" % (min_p,))
+    if kv_bits and not use_cache:
+        raise ValueError("kv_bits quantises the KV cache: it needs use_cache")
 
     cache_ok = bool(use_cache) and varying_condition is None
     sess = None
@@ -147,7 +153,7 @@ def generate(model, maps, device, out_dir, conditioning, short_filename=False,
 
             if cache_ok and T <= max_input_len:
                 # ---- incremental path: absolute positions are stable
-                if (top_k != 1 and V <= 4096 and device_loop and sess is not None and fed == T - 1 and gen_len - i >= 2
+                if (top_k != 1 and device_loop and sess is not None and fed == T - 1 and gen_len - i >= 2
                         and max_input_len - T >= 2):
                     # ---- the rest of the cache-valid span entirely on the device (DecodeSession.sample_run): the
                     # uniforms are drawn here, one torch.rand(batch_size) per step exactly like the eager loop below, so
@@ -155,14 +161,14 @@ def generate(model, maps, device, out_dir, conditioning, short_filename=False,
                     n_dev = min(gen_len - i + 1, max_input_len - T + 1)
                     uni = torch.stack([torch.rand(batch_size, device=device) for _ in range(n_dev)])
                     ids_dev = sess.sample_run(gen_song[fed], n_dev, conditions_tensor, specials, is_timeshift, repeat_counts,
-                                              temp_note, temp_rest, penalty_coeff, top_k, top_p, uni)      # [B, n_dev]
+                                              temp_note, temp_rest, penalty_coeff, top_k, top_p, uni, min_p=min_p)      # [B, n_dev]
                     fed += n_dev
                     gen_song = torch.cat((gen_song, ids_dev[:, :n_dev - 1].t()), 0)
                     gen_inds = ids_dev[:, n_dev - 1].clone()[None, :]
                     i += n_dev - 1
                     continue
                 if sess is None:
-                    sess = DecodeSession(model, batch_size)
+                    sess = DecodeSession(model, batch_size, kv_bits=kv_bits)
                     if conditioning == "continuous_token":
                         sess.prefill_condition_slots(conditions_tensor)
                     elif conditioning == "discrete_token":
@@ -199,7 +205,10 @@ def generate(model, maps, device, out_dir, conditioning, short_filename=False,
             lg = output.float()
             lg = lg if lg.is_contiguous() else lg.contiguous()
             uni = torch.rand(batch_size, device=device)
-            ops.sample_topk_topp(lg, V, specials, temp.float().contiguous(), top_k, top_p, uni, picked, n_choices_buf)
+            if min_p > 0 or V > 4096:
+                ops.sample_minp(lg, V, specials, temp.float().contiguous(), top_k, top_p, min_p, uni, picked, n_choices_buf)
+            else:
+                ops.sample_topk_topp(lg, V, specials, temp.float().contiguous(), top_k, top_p, uni, picked, n_choices_buf)
             gen_inds = picked.clone()[None, :]
             n_choices = n_choices_buf
             repeat_counts = update_repeat_counts(repeat_counts, n_choices)
@@ -253,6 +262,8 @@ def main():
     parser.add_argument('--temp', type=float, nargs='+', default=[1.2, 1.2])
     parser.add_argument('--topk', type=int, default=-1)
     parser.add_argument('--topp', type=float, default=0.7)
+    parser.add_argument('--minp', type=float, default=0.0, help="drop tokens less likely than this share of the most likely one (0: off)")
+    parser.add_argument('--kv_bits', type=int, default=None, choices=[4, 8], help="hold the KV cache in 4 or 8 bits (default: the model's own type)")
     parser.add_argument('--debug', action='store_true')
     parser.add_argument('--seed', type=int, default=0)
     parser.add_argument('--no_amp', action='store_true', help="run the exact-f32 tier instead of a 16-bit one")
@@ -277,6 +288,10 @@ def main():
     assert len(args.valence) == len(args.arousal), "Lengths of valence and arousal must be equal"
     assert (args.conditioning == "none") == (args.valence == [None] or args.arousal == [None]), \
         "If conditioning is used, specify valence and arousal; if not, don't"
+    if args.kv_bits and args.no_cache:
+        parser.error("--kv_bits quantises the KV cache: it does not go with --no_cache")
+    if not 0 <= args.minp <= 1:
+        parser.error("--minp must lie in [0, 1]")
     if args.no_cuda or not torch.cuda.is_available():
         raise SystemExit("generate.py: the MI355X engine needs a HIP device (no CPU fallback)")
     if args.seed > 0:
@@ -329,7 +344,7 @@ def main():
                 gen_len=args.gen_len, max_input_len=args.max_input_len, amp=not args.no_amp, primers=p_run,
                 temperatures=args.temp, top_k=args.topk, debug=args.debug, verbose=not args.quiet, seed=args.seed,
                 use_cache=not args.no_cache, device_loop=not args.no_device_loop,
-                use_window_graph=not args.no_window_graph)
+                use_window_graph=not args.no_window_graph, min_p=args.minp, kv_bits=args.kv_bits)
 
 
 if __name__ == '__main__':

@@ -22,20 +22,30 @@ position shifts by one (generate.py:101-103 + music_multi.py:163) and
 `continuous_concat` with a per-step varying condition changes every cached
 embedding; in both cases the caller falls back to full recompute (exact
 reference semantics) -- see generate.py.
+
+`kv_bits` = 4 or 8 holds the caches quantised (kvcache.QuantKVCache: 34 / 66 bytes per row of 64 values instead of 128 in bf16): the
+projection leaves the new rows in a staging row, me_kvq_write quantises them into place and me_kvq_attn reads the codes as they lie;
+its partial records are the ones me_dec_proj_resid joins, everything else of the step is unchanged.
 """
 import os
 
 import torch
 
 from . import ops
+from .kvcache import HEAD_DIMS, QuantKVCache
 
 ROWS = 8            # sequences per kernel call (me_dec_*: Mr <= 8); larger batches run in row chunks
 
 
 class DecodeSession:
-    def __init__(self, model, batch_size):
+    def __init__(self, model, batch_size, kv_bits=None):
+        """kv_bits: None = caches in the model's compute type; 4 / 8 = quantised caches."""
         if model.training:
             raise RuntimeError("DecodeSession needs model.eval()")
+        if kv_bits not in (None, 4, 8):
+            raise ValueError("kv_bits must be None, 4 or 8 (got %r)" % (kv_bits,))
+        if kv_bits and (model.dh not in HEAD_DIMS or model.max_seq % 32):
+            raise RuntimeError("quantised caches need a head dim of 32, 48 or 64 and max_seq in whole blocks of 32 (got %d, %d)" % (model.dh, model.max_seq))
         self.m = model
         self.B = int(batch_size)
         m = model
@@ -44,8 +54,13 @@ class DecodeSession:
         B = self.B
         e = lambda *s, dtype=dt: torch.empty(*s, dtype=dtype, device=dev)
         f32 = torch.float32
-        self.kc = [torch.zeros(B, H, m.max_seq, dh, dtype=dt, device=dev) for _ in range(m.num_layer)]
-        self.vc = [torch.zeros(B, H, m.max_seq, dh, dtype=dt, device=dev) for _ in range(m.num_layer)]
+        self.kv_bits = kv_bits
+        if kv_bits:
+            self.kvq = [QuantKVCache(B, H, m.max_seq, dh, kv_bits, dev) for _ in range(m.num_layer)]
+            self.knew, self.vnew = e(B, H, 1, dh), e(B, H, 1, dh)          # a step's rows before they are quantised
+        else:
+            self.kc = [torch.zeros(B, H, m.max_seq, dh, dtype=dt, device=dev) for _ in range(m.num_layer)]
+            self.vc = [torch.zeros(B, H, m.max_seq, dh, dtype=dt, device=dev) for _ in range(m.num_layer)]
         self.xlo = dt != f32                                   # bf16 tier: condition slots are fed as hi + lo rows
         self.q, self.hid = e(B, d), e(B, di)
         self.xres, self.o1res = e(B, d, dtype=f32), e(B, d, dtype=f32)     # f32 residual inputs (LayerNorm outputs)
@@ -60,7 +75,7 @@ class DecodeSession:
         # fused qkv + attention stage (me_dec_ln_qkv_attn): the last split is the new key, so it needs >= 2 splits
         # (the kernel's own preconditions, me_dec_ln_qkv_attn / me_dec_embed_qkv_attn: d % 8 == 0, d <= 1024, dh in {32, 48, 64};
         # any other shape takes the separate me_dec_qkv + me_dec_attn launches)
-        self.fused = os.environ.get("MIDIEMO_DEC_UNFUSED", "0") in ("", "0") and d <= 1024 and d % 8 == 0 and dh in (32, 48, 64) and \
+        self.fused = not kv_bits and os.environ.get("MIDIEMO_DEC_UNFUSED", "0") in ("", "0") and d <= 1024 and d % 8 == 0 and dh in (32, 48, 64) and \
             self.nsplit >= 2 and -(-m.max_seq // (self.nsplit - 1)) <= 2048
         self.logits = e(B, V, dtype=f32)
         # One persistent launch per token (me_dec_token, round 6) instead of 4 per layer + head: the stages exchange self-validating
@@ -118,6 +133,8 @@ class DecodeSession:
             if self._pos_dev is None:
                 self.t += 1
             return self.logits
+        if self.kv_bits:
+            return self._layers_and_head_quantised(tokens, cond, cw, cb, x_hi, x_lo)
         for r0 in range(0, B, ROWS):                          # row chunks (Mr <= 8 per kernel call)
             r1 = min(B, r0 + ROWS)
             Mr = r1 - r0
@@ -169,11 +186,56 @@ class DecodeSession:
             self.t += 1
         return self.logits
 
+    def _layers_and_head_quantised(self, tokens, cond, cw, cb, x_hi, x_lo):
+        """The same position over quantised caches.  The projections go in chunks of 8 rows, cache and attention take the whole batch."""
+        m, B, t = self.m, self.B, self.t
+        d, di, H, dh, V = m.embedding_dim, m.d_inner, m.num_head, m.dh, m.vocab_size
+        f, dt, eps, ns = m.flat_params, m.compute_dtype, m.LN_EPS, self.nsplit
+        pv = lambda name: m._pview(f, name)
+        chunks = [(r0, min(B, r0 + ROWS)) for r0 in range(0, B, ROWS)]
+        pos = self._pos_dev if self._pos_dev is not None else t
+        if tokens is not None:
+            # the embedding row of the fed token as hi + lo, like the condition slots (me_dec_embed_qkv would append to a cache of type T)
+            x_hi = torch.empty(B, d, dtype=dt, device=f.device)
+            x_lo = torch.empty_like(x_hi) if self.xlo else None
+            ops.embed_fwd(x_hi, tokens, cond if cw is not None else None, pv("embedding.weight"), cw, cb, None, None, m._pe if self._pos_dev is not None else m._pe[t:],
+                          ops.ME_COND_CONCAT if cw is not None else ops.ME_COND_NONE, B, 1, d, m.d_condition if cw is not None else 0, 0.0, 0,
+                          pos_dev=self._pos_dev, out_lo=x_lo)
+        k_rows, v_rows = self.knew.transpose(1, 2), self.vnew.transpose(1, 2)
+        for i in range(m.num_layer):
+            W, p, pp = m._prep["layers"][i], f"enc_layers.{i}.", f"enc_layers.{i - 1}."
+            for r0, r1 in chunks:
+                first = (None, None, None, eps, x_hi[r0:r1], x_lo[r0:r1] if x_lo is not None else None)
+                later = (self.s2[r0:r1], pv(pp + "layernorm2.weight"), pv(pp + "layernorm2.bias"), eps, None, None) if i else None
+                ops.dec_qkv(*(later or first), W["Wqkv"], W["bqkv"], self.xres[r0:r1], self.q[r0:r1], self.knew[r0:r1], self.vnew[r0:r1],
+                            r1 - r0, d, H, dh, 1, 0, None, dt)
+            c = self.kvq[i]
+            ops.kvq_write(k_rows, v_rows, c.k, c.k_scale, c.v, c.v_scale, c.bits, pos)
+            ops.kvq_attn(self.q.view(B, H, dh), c.k, c.k_scale, c.v, c.v_scale, None, c.bits, pos, W["E"], None, self.part, ns)
+            for r0, r1 in chunks:
+                Mr = r1 - r0
+                ops.dec_proj_resid(self.part[r0 * H:r1 * H], ns, H, dh, None, W["Wo"], pv(p + "rga.fc.bias"), self.xres[r0:r1], self.s1[r0:r1],
+                                   Mr, d, d, dt)
+                ops.dec_ln_proj(self.s1[r0:r1], pv(p + "layernorm1.weight"), pv(p + "layernorm1.bias"), eps, W["W1"],
+                                pv(p + "FFN_pre.bias"), self.o1res[r0:r1], self.hid[r0:r1], Mr, di, d, ops.ME_EPI_RELU, dt)
+                ops.dec_proj_resid(None, 0, 0, 0, self.hid[r0:r1], W["W2"], pv(p + "FFN_suf.bias"), self.o1res[r0:r1],
+                                   self.s2[r0:r1], Mr, d, di, dt)
+        pl = f"enc_layers.{m.num_layer - 1}."
+        for r0, r1 in chunks:
+            ops.dec_ln_proj(self.s2[r0:r1], pv(pl + "layernorm2.weight"), pv(pl + "layernorm2.bias"), eps,
+                            m._prep["head"]["Wf"], pv(m._HEAD_B), None, self.logits[r0:r1], r1 - r0, V, d, ops.ME_EPI_OUT_F32, dt)
+        if self._pos_dev is None:
+            self.t += 1
+        return self.logits
+
     # -------------------------------------------------------------- public steps
     @property
     def launches_per_token(self):
         if self.token_kernel:
             return 2                                                # the token + pick / commit
+        if self.kv_bits:
+            chunks = -(-self.B // ROWS)
+            return (2 + 4 * chunks) * self.m.num_layer + 1 + chunks + 1     # + embedding, head, pick / commit
         return (4 if self.fused else 5) * self.m.num_layer + 2     # + head, + pick / commit
 
     def check_token_status(self):
@@ -275,19 +337,23 @@ class DecodeSession:
         return self._hist[:, t0:t0 + n_steps]
 
     def sample_run(self, tokens, n_steps, cond, special, is_timeshift, repeat_counts, temp_note, temp_rest,
-                   penalty_coeff, top_k, top_p, uniforms, use_graph=True):
+                   penalty_coeff, top_k, top_p, uniforms, use_graph=True, min_p=0.0):
         """The sampling loop of generate() (generate.py:99-189) on the device: feed `tokens` (int64 [B]) at the next
         position, sample the next token with me_sample_step (NaN / specials mask, log-softmax, the per-row temperature
         with its repeat penalty, top-k, nucleus cut, inverse-CDF draw at uniforms[step], repeat-counter update), append
         it and feed it back, n_steps times.  One HIP graph per token (33 launches) instead of ~40 eager launches and a
         dozen small torch ops from Python.  `uniforms` float32 [n_steps, B] are drawn by the caller (so the random
-        stream is the caller's generator's); `repeat_counts` float32 [B] is updated in place.
+        stream is the caller's generator's); `repeat_counts` float32 [B] is updated in place.  `min_p` > 0 drops tokens less likely than
+        min_p times the most likely one; it, and vocabularies of more than 4096 symbols, are served by me_sample_minp_step.
         Returns the sampled ids int64 [B, n_steps] (on the device)."""
         m = self.m
         dev = m.flat_params.device
         n_steps = int(n_steps)
-        if m.vocab_size > 4096:
-            raise RuntimeError("sample_run: the sampling kernel sorts at most 4096 logits (vocab %d)" % m.vocab_size)
+        wide = min_p > 0 or m.vocab_size > 4096
+        if m.vocab_size > ops._lib.ME_SAMPLE_MAX_VOCAB:
+            raise RuntimeError("sample_run: the sampling kernels take at most %d symbols (vocab %d)" % (ops._lib.ME_SAMPLE_MAX_VOCAB, m.vocab_size))
+        if not 0 <= min_p <= 1:
+            raise ValueError("min_p must lie in [0, 1] (got %r)" % (min_p,))
         if self.t + n_steps > m.max_seq:
             raise RuntimeError("decode positions %d..%d exceed max_seq %d" % (self.t, self.t + n_steps, m.max_seq))
         if uniforms.shape[0] < n_steps or uniforms.shape[1] != self.B or uniforms.dtype != torch.float32:
@@ -312,7 +378,7 @@ class DecodeSession:
         self._s_ts.copy_(is_timeshift.to(device=dev, dtype=torch.uint8))
         sp = None if special is None else special.to(device=dev, dtype=torch.int32).contiguous()
         # everything that is baked into the captured step: scalars, the special-id list and the position origin
-        key = (float(temp_note), float(temp_rest), float(penalty_coeff), int(top_k), float(top_p), self.t,
+        key = (float(temp_note), float(temp_rest), float(penalty_coeff), int(top_k), float(top_p), float(min_p), self.t,
                None if sp is None else tuple(sp.tolist()))
         if key != self._s_key:
             self._s_key, self._s_graph, self._s_special = key, None, sp
@@ -323,8 +389,12 @@ class DecodeSession:
             try:
                 self._embed_and_run(self._tok, self._cond if m.d_condition > 0 else None)
                 # block b reads the fed token of row b first and writes the sampled one last: the input buffer is reused
-                ops.sample_step(self.logits, m.vocab_size, self._s_special, self._tok, self._s_ts, self._s_rc, temp_note,
-                                temp_rest, penalty_coeff, top_k, top_p, self._s_u, self._pos, t0, self._tok)
+                if wide:
+                    ops.sample_minp_step(self.logits, m.vocab_size, self._s_special, self._tok, self._s_ts, self._s_rc, temp_note,
+                                         temp_rest, penalty_coeff, top_k, top_p, min_p, self._s_u, self._pos, t0, self._tok)
+                else:
+                    ops.sample_step(self.logits, m.vocab_size, self._s_special, self._tok, self._s_ts, self._s_rc, temp_note,
+                                    temp_rest, penalty_coeff, top_k, top_p, self._s_u, self._pos, t0, self._tok)
                 ops.decode_commit(self._tok, self._hist, self._pos, self.B)         # history[pos] = next; ++pos
             finally:
                 self._pos_dev = None
