@@ -474,14 +474,18 @@ int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
  *   `part` (me_workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh, dtype) bytes, 16-byte aligned, uninitialised, private to the
  *   call until it has run) holds the ranges' records and a second launch joins them in ascending order.  out = NULL: the records are the
  *   result, as me_dec_attn leaves them (nsplit <= 8: me_dec_proj_resid joins them; it takes a row without keys for NaN). */
-int me_kvq_write(const void* k, const void* v, const int64_t* strides, void* kcodes, void* kscale, void* vcodes, void* vscale, int B, int n,
-                 int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, const int32_t* lens, int dtype, void* stream);
-int me_kvq_read(const void* kcodes, const void* kscale, const void* vcodes, const void* vscale, void* k, void* v, const int64_t* strides, int B,
-                int n, int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, const int32_t* lens, int dtype, void* stream);
+typedef struct me_kvq_cache {       /* HOST struct, read during the call */
+    void* kcodes; void* kscale; void* vcodes; void* vscale;
+    int32_t B, H, dh, blocks, bits;
+} me_kvq_cache;
+int me_kvq_write(const me_kvq_cache* c, const void* k, const void* v, const int64_t* strides, int n, int t, const int32_t* t_dev, int ld_t,
+                 const int32_t* lens, int dtype, void* stream);
+int me_kvq_read(const me_kvq_cache* c, void* k, void* v, const int64_t* strides, int n, int t, const int32_t* t_dev, int ld_t, const int32_t* lens,
+                int dtype, void* stream);
 int me_kvq_splits(int B, int H, int tokens);
-int me_kvq_attn(const void* q, int64_t ldq_b, int64_t ldq_h, const void* kcodes, const void* kscale, const void* vcodes, const void* vscale,
-                const void* E, int M, const uint8_t* key_pad, int ld_pad, void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes,
-                int nsplit, int B, int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, int dtype, void* stream);
+int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* E, int M, const uint8_t* key_pad, int ld_pad,
+                void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes, int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype,
+                void* stream);
 
 /* Greedy pick for generate(top_k=1): logits f32 [B, ld]; NaN -> 0, ids in
  * special[0..n_special) -> -inf, argmax -> out_ids[B] (generate.py:122-136,166-183). */

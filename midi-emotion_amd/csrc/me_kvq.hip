@@ -58,13 +58,14 @@ struct RowArgs {                                              // k / v rows [B][
     void* k; void* v;
     int64_t skb, skn, skh, svb, svn, svh;
     uint8_t* kc; u16* ks; uint8_t* vc; u16* vs;
-    int n, H, blocks, t, ld_t, vec;
+    int n, H, blocks, t, ld_t;
     const int32_t* t_dev; const int32_t* lens;
 };
 
-template <typename T> ME_DEV void load8(float (&x)[8], const T* p, bool vec) {
-    if (vec) {
-        constexpr int CH = ET<T>::CH;
+// 8 elements of a row: VEC = two (four) 16-byte accesses, for rows that are 16-byte aligned throughout
+template <typename T, bool VEC> ME_DEV void load8(float (&x)[8], const T* p) {
+    constexpr int CH = ET<T>::CH;
+    if constexpr (VEC) {
 #pragma unroll
         for (int u = 0; u < 8 / CH; ++u) {
             const chunk16 c = ld_chunk(p + u * CH);
@@ -77,20 +78,18 @@ template <typename T> ME_DEV void load8(float (&x)[8], const T* p, bool vec) {
         for (int i = 0; i < 8; ++i) x[i] = ET<T>::to_f(p[i]);
     }
 }
-template <typename T> ME_DEV void store8(T* p, const float (&x)[8], bool vec) {
-    if (vec) {
-        constexpr int CH = ET<T>::CH;
-#pragma unroll
-        for (int u = 0; u < 8 / CH; ++u) {
-            chunk16 c;
-            T* e = reinterpret_cast<T*>(&c);
-#pragma unroll
-            for (int i = 0; i < CH; ++i) e[i] = ET<T>::from_f(x[u * CH + i]);
-            st_chunk(p + u * CH, c);
-        }
-    } else {
+template <typename T, bool VEC> ME_DEV void store8(T* p, const float (&x)[8]) {
+    if constexpr (!VEC) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = ET<T>::from_f(x[i]);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4_t*>(p) = (f32x4_t){x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4_t*>(p + 4) = (f32x4_t){x[4], x[5], x[6], x[7]};
+    } else {
+        typename V16<T>::x8 v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (T)x[i];
+        *reinterpret_cast<typename V16<T>::x8*>(p) = v;
     }
 }
 
@@ -146,7 +145,7 @@ template <int BITS, bool WIDE> ME_DEV void quantise8(const float (&x)[8], u16& s
 // lane); V changes its order through LDS (8 tokens of a dimension per thread), and a group of 8 tokens that the call covers only in
 // part keeps its other codes (read, merged, written by the one thread that owns the word).
 // ---------------------------------------------------------------------------------------------------------
-template <typename T, int BITS, int DH>
+template <typename T, int BITS, int DH, bool VEC>
 __global__ __launch_bounds__(256) void kvq_write_kernel(const RowArgs a) {
     constexpr int W = BITS == 4 ? 1 : 2;
     __shared__ uint32_t vq[KB][8 * W];
@@ -164,8 +163,8 @@ __global__ __launch_bounds__(256) void kvq_write_kernel(const RowArgs a) {
     for (int i = 0; i < 8; ++i) { xk[i] = 0.f; xv[i] = 0.f; }
     if (active) {
         const int64_t i = j - t;
-        load8<T>(xk, reinterpret_cast<const T*>(a.k) + (int64_t)b * a.skb + i * a.skn + (int64_t)h * a.skh + d0, a.vec);
-        load8<T>(xv, reinterpret_cast<const T*>(a.v) + (int64_t)b * a.svb + i * a.svn + (int64_t)h * a.svh + d0, a.vec);
+        load8<T, VEC>(xk, reinterpret_cast<const T*>(a.k) + (int64_t)b * a.skb + i * a.skn + (int64_t)h * a.skh + d0);
+        load8<T, VEC>(xv, reinterpret_cast<const T*>(a.v) + (int64_t)b * a.svb + i * a.svn + (int64_t)h * a.svh + d0);
     }
     u16 sk, sv;
     uint32_t ck[2], cv[2];
@@ -226,7 +225,7 @@ template <int BITS> ME_DEV void expand8(float (&x)[8], uint32_t c0, uint32_t c1,
 }
 ME_DEV float bf16_bits(u16 u) { return __uint_as_float((uint32_t)u << 16); }
 
-template <typename T, int BITS, int DH>
+template <typename T, int BITS, int DH, bool VEC>
 __global__ __launch_bounds__(256) void kvq_read_kernel(const RowArgs a) {
     constexpr int W = BITS == 4 ? 1 : 2;
     __shared__ uint32_t vq[8][8][4 * W];                      // [d % 8][d / 8][tokens]: the 8 lanes of a row read 8 different banks
@@ -276,21 +275,23 @@ __global__ __launch_bounds__(256) void kvq_read_kernel(const RowArgs a) {
         }
     }
     if (i < 0 || i >= a.n || d0 >= DH) return;
-    store8<T>(reinterpret_cast<T*>(a.k) + (int64_t)b * a.skb + i * a.skn + (int64_t)h * a.skh + d0, xk, a.vec);
-    store8<T>(reinterpret_cast<T*>(a.v) + (int64_t)b * a.svb + i * a.svn + (int64_t)h * a.svh + d0, xv, a.vec);
+    store8<T, VEC>(reinterpret_cast<T*>(a.k) + (int64_t)b * a.skb + i * a.skn + (int64_t)h * a.skh + d0, xk);
+    store8<T, VEC>(reinterpret_cast<T*>(a.v) + (int64_t)b * a.svb + i * a.svn + (int64_t)h * a.svh + d0, xv);
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// attention: one wave per head, blocks of up to 8 heads of one sequence, keys in tiles of 128, split over grid.x
+// attention: a block is up to 8 waves = heads x key ranges of one sequence; keys in tiles of 128, a head's ranges take them in turn and
+// meet in LDS at the end; grid.x may cut the keys further
 //   s_j = (q.k_j + q.E[M-1-(t-j)]) / sqrt(dh);  running maximum and sum in base 2, 32 bits
 //   K: two MFMAs give a lane the four row products of ONE key (rows 4 g + i of the result: digit i, and A's zero blocks pick
 //      the chunk that belongs to the row's 16 keys); V: the weights p_j * scale_j (4 bits: scaled by a power of two per tile) are the rows.
-//   E is shared by the heads: its products for 512 keys x 8 heads come from one matrix product per 16 keys and wait in LDS.
+//   E is shared by a block's heads: its products for a stretch of keys come from one matrix product per 16 keys and wait in LDS.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int RELK = 512;                                     // keys per stretch of relative logits
+constexpr int RELS = 4096;                                    // relative logits in LDS: a stretch of RELS / (heads of the block) keys
 constexpr int TK = 128;                                       // keys per tile
 template <int BITS> constexpr int PROW = BITS == 4 ? TK + 16 : 2 * TK + 16;   // bytes between the parts in LDS (16 more than the row: other banks)
-constexpr int HG = 8;                                         // heads per block
+constexpr int WAVES = 8;                                      // waves of a block at most: heads x key ranges, both powers of two
+constexpr int HG = 8;                                         // heads of a block at most
 
 struct AttnArgs {
     const void* q; int64_t sqb, sqh;
@@ -299,7 +300,7 @@ struct AttnArgs {
     const uint8_t* pad; int ld_pad;
     void* out; int64_t sob, soh;
     float* part; int nsplit;
-    int H, blocks, t, ld_t;
+    int H, blocks, t, ld_t, hpb, kw;
     const int32_t* t_dev;
     float scale;
     float munit;                                              // unit of a record's maximum: 1 = base 2 (kvq_join_kernel), ln 2 = natural
@@ -380,7 +381,7 @@ template <int DH> ME_DEV int slot_dim(int r, int sg, int i) {
 }
 
 template <typename T, int BITS, int DH, bool REL>
-__global__ __launch_bounds__(64 * HG) void kvq_attn_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) {
     constexpr bool WIDE = sizeof(T) == 4;
     constexpr int NP = BITS == 4 ? (WIDE ? 6 : 4) : (WIDE ? 3 : 2);               // digits / bfloat16 parts of a weight
     constexpr int NQ = BITS == 4 ? NP : (WIDE ? 3 : (__is_same(T, bf16_t) ? 1 : 2));      // and of a query element (16-bit types: exact in parts)
@@ -388,12 +389,14 @@ __global__ __launch_bounds__(64 * HG) void kvq_attn_kernel(const AttnArgs a) {
     constexpr int PR = PROW<BITS>;
     constexpr float LOG2E = 1.4426950408889634f;
     __shared__ float qs[HG][DH];
-    __shared__ __attribute__((aligned(16))) uint8_t parts[HG][NP * PR];
-    __shared__ float rel[REL ? HG : 1][REL ? RELK : 1];
+    __shared__ __attribute__((aligned(16))) uint8_t parts[WAVES][NP * PR];
+    __shared__ float rel[REL ? RELS : 1];
+    __shared__ float jm[WAVES], jl[WAVES], jo[WAVES][DH];     // key ranges of a head meet here
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
     const int c = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x, b = blockIdx.z, h0 = blockIdx.y * HG, nh = min(HG, a.H - h0);
-    const int hh = min(wid, nh - 1), h = h0 + hh;             // waves past the last head repeat it and store nothing
+    const int hpb = a.hpb, kw = a.kw, hw = wid / kw, wk = wid % kw;
+    const int split = blockIdx.x, b = blockIdx.z, h0 = blockIdx.y * hpb, nh = min(hpb, a.H - h0);
+    const int hh = min(hw, nh - 1), h = h0 + hh;              // waves past the last head repeat it and store nothing
     int n = min(pos_of(a.t, a.t_dev, a.ld_t, b), a.blocks * KB - 1) + 1;
     if (REL) n = min(n, a.M);
     n = max(n, 0);
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(64 * HG) void kvq_attn_kernel(const AttnArgs a) {
     const uint8_t* pad = a.pad ? a.pad + (size_t)b * a.ld_pad : nullptr;
 
     Tile<BITS, DH> cur;
-    if (j0 < j1) load_tile<BITS, DH>(cur, kc, vc, ks, vs, pad, a.ld_pad, j0, j1, lane);       // in flight under the query's preparation
+    if (j0 + wk * TK < j1) load_tile<BITS, DH>(cur, kc, vc, ks, vs, pad, a.ld_pad, j0 + wk * TK, j1, lane);       // in flight under the query's preparation
 
     for (int i = tid; i < nh * DH; i += nw * 64)
         qs[i / DH][i % DH] = ET<T>::to_f(reinterpret_cast<const T*>(a.q)[(int64_t)b * a.sqb + (int64_t)(h0 + i / DH) * a.sqh + i % DH]);
@@ -474,8 +477,9 @@ __global__ __launch_bounds__(64 * HG) void kvq_attn_kernel(const AttnArgs a) {
     for (int u = 0; u < DH / 16; ++u) acc[u] = 0.f;
     const float cs = a.scale * LOG2E, cq = cs * qinv;
 
-    for (int c0 = j0; c0 < j1; c0 += REL ? RELK : j1 - j0) {
-        const int c1 = REL ? min(c0 + RELK, j1) : j1;
+    const int stretch = REL ? RELS / hpb : max(j1 - j0, 1);   // a multiple of kw tiles
+    for (int c0 = j0; c0 < j1; c0 += stretch) {
+        const int c1 = min(c0 + stretch, j1);
         if constexpr (REL) {
             const int t = n - 1;
             __syncthreads();                                  // the last stretch has been read
@@ -501,13 +505,14 @@ __global__ __launch_bounds__(64 * HG) void kvq_attn_kernel(const AttnArgs a) {
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (4 * g + i < nh) rel[4 * g + i][kt + c] = d[i];
+                for (int i = 0; i < 4; ++i) if (4 * g + i < nh) rel[(4 * g + i) * stretch + kt + c] = d[i];
             }
             __syncthreads();
         }
-        for (int jt = c0; jt < c1; jt += TK) {
+        for (int jt = c0 + wk * TK; jt < c1; jt += kw * TK) {
             Tile<BITS, DH> nxt;
-            if (jt + TK < j1) load_tile<BITS, DH>(nxt, kc, vc, ks, vs, pad, a.ld_pad, jt + TK, j1, lane);
+            const bool more = jt + kw * TK < j1;
+            if (more) load_tile<BITS, DH>(nxt, kc, vc, ks, vs, pad, a.ld_pad, jt + kw * TK, j1, lane);
             // ---- logits of keys jt + lane and jt + 64 + lane
             float s[2];
 #pragma unroll
@@ -540,7 +545,7 @@ __global__ __launch_bounds__(64 * HG) void kvq_attn_kernel(const AttnArgs a) {
                     for (int i = 1; i < NQ; ++i) v += d[i];
                 }
                 v *= bf16_bits(cur.ks[u]) * cq;
-                if constexpr (REL) v = fmaf(rel[hh][jt - c0 + 64 * u + lane], cs, v);
+                if constexpr (REL) v = fmaf(rel[hh * stretch + jt - c0 + 64 * u + lane], cs, v);
                 s[u] = cur.pad[u] ? -INFINITY : v;
             }
             // ---- running softmax
@@ -619,11 +624,29 @@ __global__ __launch_bounds__(64 * HG) void kvq_attn_kernel(const AttnArgs a) {
                     acc[u] = fmaf(acc[u], alpha, v);
                 }
             }
-            if (jt + TK < j1) cur = nxt;
+            if (more) cur = nxt;
         }
     }
-    const float l = wave_sum(lsum);
-    if (wid >= nh) return;
+    float l = wave_sum(lsum);
+    if (kw > 1) {                                             // join the head's key ranges, in ascending order
+        if (lane == 0) { jm[wid] = m; jl[wid] = l; }
+#pragma unroll
+        for (int u = 0; u < DH / 16; ++u) if (lane < 16) jo[wid][16 * u + lane] = acc[u];
+        __syncthreads();
+        if (wk != 0) return;
+        for (int i = 1; i < kw; ++i) m = fmaxf(m, jm[wid + i]);
+        const float ms = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+#pragma unroll
+        for (int u = 0; u < DH / 16; ++u) acc[u] = 0.f;
+        for (int i = 0; i < kw; ++i) {
+            const float w = __builtin_amdgcn_exp2f(jm[wid + i] - ms);
+            l = fmaf(w, jl[wid + i], l);
+#pragma unroll
+            for (int u = 0; u < DH / 16; ++u) acc[u] = fmaf(w, jo[wid + i][16 * u + (lane & 15)], acc[u]);
+        }
+    }
+    if (hw >= nh) return;
     if (a.part) {
         float* rec = a.part + (bh * a.nsplit + split) * ME_DEC_PART_REC(DH);
         if (lane == 0) *reinterpret_cast<f32x4_t*>(rec) = (f32x4_t){m * a.munit, l, 0.f, 0.f};
@@ -655,36 +678,45 @@ __global__ __launch_bounds__(256) void kvq_join_kernel(const float* __restrict__
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <typename T, int BITS> void launch_rows(bool write, int dh, dim3 grid, hipStream_t st, const RowArgs& a) {
+template <typename T, int BITS, int DH> void launch_rows(bool write, bool vec, dim3 grid, hipStream_t st, const RowArgs& a) {
     if (write) {
-        if (dh == 32) kvq_write_kernel<T, BITS, 32><<<grid, 256, 0, st>>>(a);
-        else if (dh == 48) kvq_write_kernel<T, BITS, 48><<<grid, 256, 0, st>>>(a);
-        else kvq_write_kernel<T, BITS, 64><<<grid, 256, 0, st>>>(a);
+        if (vec) kvq_write_kernel<T, BITS, DH, true><<<grid, 256, 0, st>>>(a);
+        else kvq_write_kernel<T, BITS, DH, false><<<grid, 256, 0, st>>>(a);
     } else {
-        if (dh == 32) kvq_read_kernel<T, BITS, 32><<<grid, 256, 0, st>>>(a);
-        else if (dh == 48) kvq_read_kernel<T, BITS, 48><<<grid, 256, 0, st>>>(a);
-        else kvq_read_kernel<T, BITS, 64><<<grid, 256, 0, st>>>(a);
+        if (vec) kvq_read_kernel<T, BITS, DH, true><<<grid, 256, 0, st>>>(a);
+        else kvq_read_kernel<T, BITS, DH, false><<<grid, 256, 0, st>>>(a);
     }
 }
+template <typename T, int BITS> void launch_rows(bool write, bool vec, int dh, dim3 grid, hipStream_t st, const RowArgs& a) {
+    if (dh == 32) launch_rows<T, BITS, 32>(write, vec, grid, st, a);
+    else if (dh == 48) launch_rows<T, BITS, 48>(write, vec, grid, st, a);
+    else launch_rows<T, BITS, 64>(write, vec, grid, st, a);
+}
 
-int rows_call(bool write, void* k, void* v, const int64_t* stride, uint8_t* kc, void* ks, uint8_t* vc, void* vs, int B, int n, int H, int dh,
-              int blocks, int bits, int t, const int32_t* t_dev, int ld_t, const int32_t* lens, int dtype, hipStream_t st) {
+int cache_status(const me_kvq_cache* c) {
+    if (!c || !c->kcodes || !c->kscale || !c->vcodes || !c->vscale) return ME_ERR_NULL;
+    if ((c->dh != 32 && c->dh != 48 && c->dh != 64) || (c->bits != 4 && c->bits != 8) || c->B < 0 || c->H < 0 || c->blocks < 0 || c->blocks > (1 << 25) ||
+        c->B > 65535 || c->H > 65535) return ME_ERR_BAD_SHAPE;
+    return aligned16(c->kcodes) && aligned16(c->vcodes) ? ME_OK : ME_ERR_ALIGNMENT;
+}
+
+int rows_call(bool write, const me_kvq_cache* c, void* k, void* v, const int64_t* stride, int n, int t, const int32_t* t_dev, int ld_t,
+              const int32_t* lens, int dtype, hipStream_t st) {
     me_clear_error();
-    if (!k || !v || !kc || !ks || !vc || !vs) return ME_ERR_NULL;
+    if (!k || !v || !stride) return ME_ERR_NULL;
+    if (int rc = cache_status(c)) return rc;
     if (dtype != ME_F32 && dtype != ME_BF16 && dtype != ME_F16) return ME_ERR_BAD_DTYPE;
-    if ((dh != 32 && dh != 48 && dh != 64) || (bits != 4 && bits != 8) || B < 0 || n < 0 || H < 0 || blocks < 0 || blocks > (1 << 25) ||
-        B > 65535 || H > 65535 || (ld_t != 0 && ld_t != 1) || n > blocks * KB ||
-        (!t_dev && (t < 0 || (int64_t)t + n > (int64_t)blocks * KB))) return ME_ERR_BAD_SHAPE;
-    if (!aligned16(kc) || !aligned16(vc)) return ME_ERR_ALIGNMENT;
-    if (B == 0 || n == 0 || H == 0) return ME_OK;
+    if (n < 0 || (ld_t != 0 && ld_t != 1) || n > c->blocks * KB || (!t_dev && (t < 0 || (int64_t)t + n > (int64_t)c->blocks * KB))) return ME_ERR_BAD_SHAPE;
+    if (c->B == 0 || n == 0 || c->H == 0) return ME_OK;
     const int es = dtype == ME_F32 ? 4 : 2;
     bool vec = aligned16(k) && aligned16(v);
     for (int i = 0; i < 6; ++i) vec = vec && (stride[i] * es) % 16 == 0;
-    RowArgs a = {k, v, stride[0], stride[1], stride[2], stride[3], stride[4], stride[5], kc, (u16*)ks, vc, (u16*)vs, n, H, blocks, t, ld_t, vec, t_dev, lens};
+    RowArgs a = {k, v, stride[0], stride[1], stride[2], stride[3], stride[4], stride[5], (uint8_t*)c->kcodes, (u16*)c->kscale, (uint8_t*)c->vcodes,
+                 (u16*)c->vscale, n, c->H, c->blocks, t, ld_t, t_dev, lens};
     // blocks that n tokens from any position can touch (from t where it is known)
     const int nblk = t_dev ? (n + KB - 2) / KB + 1 : (t + n - 1) / KB - t / KB + 1;
-    const dim3 grid(nblk, H, B);
-#define ME_KVQ_ROWS(T) (bits == 4 ? launch_rows<T, 4>(write, dh, grid, st, a) : launch_rows<T, 8>(write, dh, grid, st, a))
+    const dim3 grid(nblk, c->H, c->B);
+#define ME_KVQ_ROWS(T) (c->bits == 4 ? launch_rows<T, 4>(write, vec, c->dh, grid, st, a) : launch_rows<T, 8>(write, vec, c->dh, grid, st, a))
     if (dtype == ME_F32) ME_KVQ_ROWS(float);
     else if (dtype == ME_BF16) ME_KVQ_ROWS(bf16_t);
     else ME_KVQ_ROWS(f16_t);
@@ -697,8 +729,8 @@ template <typename T, int BITS, int DH> void launch_attn(dim3 grid, int threads,
     else kvq_attn_kernel<T, BITS, DH, false><<<grid, threads, 0, st>>>(a);
 }
 template <typename T> void attn_call(const AttnArgs& a, int B, int dh, int bits, bool join, hipStream_t st) {
-    const dim3 grid(a.nsplit, (a.H + HG - 1) / HG, B);
-    const int threads = 64 * std::min(a.H, HG);
+    const dim3 grid(a.nsplit, (a.H + a.hpb - 1) / a.hpb, B);
+    const int threads = 64 * a.hpb * a.kw;
 #define ME_KVQ_ATTN(DHV) (bits == 4 ? launch_attn<T, 4, DHV>(grid, threads, st, a) : launch_attn<T, 8, DHV>(grid, threads, st, a))
     if (dh == 32) ME_KVQ_ATTN(32); else if (dh == 48) ME_KVQ_ATTN(48); else ME_KVQ_ATTN(64);
 #undef ME_KVQ_ATTN
@@ -714,45 +746,48 @@ template <typename T> void attn_call(const AttnArgs& a, int B, int dh, int bits,
 
 extern "C" {
 
-int me_kvq_write(const void* k, const void* v, const int64_t* strides, void* kcodes, void* kscale, void* vcodes, void* vscale, int B, int n,
-                 int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, const int32_t* lens, int dtype, void* stream) {
-    if (!strides) return ME_ERR_NULL;
-    return rows_call(true, const_cast<void*>(k), const_cast<void*>(v), strides, (uint8_t*)kcodes, kscale, (uint8_t*)vcodes, vscale, B, n, H, dh,
-                     blocks, bits, t, t_dev, ld_t, lens, dtype, (hipStream_t)stream);
+int me_kvq_write(const me_kvq_cache* c, const void* k, const void* v, const int64_t* strides, int n, int t, const int32_t* t_dev, int ld_t,
+                 const int32_t* lens, int dtype, void* stream) {
+    return rows_call(true, c, const_cast<void*>(k), const_cast<void*>(v), strides, n, t, t_dev, ld_t, lens, dtype, (hipStream_t)stream);
 }
 
-int me_kvq_read(const void* kcodes, const void* kscale, const void* vcodes, const void* vscale, void* k, void* v, const int64_t* strides, int B,
-                int n, int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, const int32_t* lens, int dtype, void* stream) {
-    if (!strides) return ME_ERR_NULL;
-    return rows_call(false, k, v, strides, (uint8_t*)const_cast<void*>(kcodes), const_cast<void*>(kscale), (uint8_t*)const_cast<void*>(vcodes),
-                     const_cast<void*>(vscale), B, n, H, dh, blocks, bits, t, t_dev, ld_t, lens, dtype, (hipStream_t)stream);
+int me_kvq_read(const me_kvq_cache* c, void* k, void* v, const int64_t* strides, int n, int t, const int32_t* t_dev, int ld_t, const int32_t* lens,
+                int dtype, void* stream) {
+    return rows_call(false, c, k, v, strides, n, t, t_dev, ld_t, lens, dtype, (hipStream_t)stream);
 }
 
+// A second launch joins the splits, so a cache is only cut where its (sequence, head) pairs leave most of the chip idle and every wave
+// keeps two tiles.
 int me_kvq_splits(int B, int H, int tokens) {
     if (B <= 0 || H <= 0 || tokens <= 0) return 1;
-    const int64_t rows = (int64_t)B * ((H + HG - 1) / HG);
-    const int64_t want = (512 + rows - 1) / rows, most = ((int64_t)tokens + TK - 1) / TK;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 64));
+    const int64_t rows = (int64_t)B * H, tiles = ((int64_t)tokens + TK - 1) / TK;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(256 / rows, tiles / (2 * WAVES)), 64));
 }
 
-int me_kvq_attn(const void* q, int64_t ldq_b, int64_t ldq_h, const void* kcodes, const void* kscale, const void* vcodes, const void* vscale,
-                const void* E, int M, const uint8_t* key_pad, int ld_pad, void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes,
-                int nsplit, int B, int H, int dh, int blocks, int bits, int t, const int32_t* t_dev, int ld_t, int dtype, void* stream) {
+int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* E, int M, const uint8_t* key_pad, int ld_pad,
+                void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes, int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype,
+                void* stream) {
     me_clear_error();
-    if (!q || !kcodes || !kscale || !vcodes || !vscale || (!out && !part)) return ME_ERR_NULL;
+    if (!q || (!out && !part)) return ME_ERR_NULL;
+    if (int rc = cache_status(c)) return rc;
     if (dtype != ME_F32 && dtype != ME_BF16 && dtype != ME_F16) return ME_ERR_BAD_DTYPE;
-    if ((dh != 32 && dh != 48 && dh != 64) || (bits != 4 && bits != 8) || B < 0 || H < 0 || blocks < 0 || blocks > (1 << 25) || B > 65535 ||
-        H > 65535 * HG || nsplit < 1 || nsplit > 64 || (ld_t != 0 && ld_t != 1) || (!t_dev && (t < -1 || t >= blocks * KB)) || (E && M < blocks * KB) ||
+    if (nsplit < 1 || nsplit > 64 || (ld_t != 0 && ld_t != 1) || (!t_dev && (t < -1 || t >= c->blocks * KB)) || (E && M < c->blocks * KB) ||
         (key_pad && ld_pad < 0)) return ME_ERR_BAD_SHAPE;
-    if (!aligned16(kcodes) || !aligned16(vcodes) || (E && !aligned16(E)) || (part && !aligned16(part))) return ME_ERR_ALIGNMENT;
-    if (B == 0 || H == 0) return ME_OK;
+    if ((E && !aligned16(E)) || (part && !aligned16(part))) return ME_ERR_ALIGNMENT;
+    if (c->B == 0 || c->H == 0) return ME_OK;
     const bool split = nsplit > 1 || !out;                    // out == NULL: the partial records are the result (me_dec_proj_resid joins them)
-    if (split && (!part || part_bytes < (size_t)B * H * nsplit * ME_DEC_PART_REC(dh) * 4)) return ME_ERR_WORKSPACE;
-    AttnArgs a = {q, ldq_b, ldq_h, (const uint8_t*)kcodes, (const u16*)kscale, (const uint8_t*)vcodes, (const u16*)vscale, E, M, key_pad, ld_pad,
-                  out, ldo_b, ldo_h, split ? part : nullptr, nsplit, H, blocks, t, ld_t, t_dev, 1.f / sqrtf((float)dh), out ? 1.f : 0.6931471805599453f};
-    if (dtype == ME_F32) attn_call<float>(a, B, dh, bits, split && out, (hipStream_t)stream);
-    else if (dtype == ME_BF16) attn_call<bf16_t>(a, B, dh, bits, split && out, (hipStream_t)stream);
-    else attn_call<f16_t>(a, B, dh, bits, split && out, (hipStream_t)stream);
+    if (split && (!part || part_bytes < (size_t)c->B * c->H * nsplit * ME_DEC_PART_REC(c->dh) * 4)) return ME_ERR_WORKSPACE;
+    // heads per block: the relative products of a stretch of keys are shared by a block's heads, so as many as leave two blocks per CU;
+    // key ranges per head: what is left of the block's 8 waves, if there are tiles for them
+    int hpb = 1, kw = 1;
+    const int64_t tiles = ((((t_dev ? (int64_t)c->blocks * KB : (int64_t)t + 1) + nsplit - 1) / nsplit) + TK - 1) / TK;
+    while (E && hpb < HG && 2 * hpb <= c->H && (int64_t)nsplit * c->B * ((c->H + 2 * hpb - 1) / (2 * hpb)) >= 512) hpb *= 2;
+    while (hpb * kw < WAVES && kw < tiles) kw *= 2;
+    AttnArgs a = {q, ldq_b, ldq_h, (const uint8_t*)c->kcodes, (const u16*)c->kscale, (const uint8_t*)c->vcodes, (const u16*)c->vscale, E, M, key_pad, ld_pad,
+                  out, ldo_b, ldo_h, split ? part : nullptr, nsplit, c->H, c->blocks, t, ld_t, hpb, kw, t_dev, 1.f / sqrtf((float)c->dh), out ? 1.f : 0.6931471805599453f};
+    if (dtype == ME_F32) attn_call<float>(a, c->B, c->dh, c->bits, split && out, (hipStream_t)stream);
+    else if (dtype == ME_BF16) attn_call<bf16_t>(a, c->B, c->dh, c->bits, split && out, (hipStream_t)stream);
+    else attn_call<f16_t>(a, c->B, c->dh, c->bits, split && out, (hipStream_t)stream);
     return me_launch_status();
 }
 

@@ -60,10 +60,10 @@ SIGNATURES = {
     "me_dec_ln_proj": [_p, _p, _p, _f, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
     "me_dec_token": [_p, _p, _p, _p, _p, _p, _i, _p, _i, _p, _i, _p, _i, _p, _i, _p, ctypes.c_size_t, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _f, _i, _i, _p],
     "me_dec_token_blocks": [_i, _i, _i, _i],
-    "me_kvq_write": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _i, _p],
-    "me_kvq_read": [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _i, _p],
+    "me_kvq_write": [_p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _p],
+    "me_kvq_read": [_p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _p],
     "me_kvq_splits": [_i, _i, _i],
-    "me_kvq_attn": [_p, _i64, _i64, _p, _p, _p, _p, _p, _i, _p, _i, _p, _i64, _i64, _p, ctypes.c_size_t, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _p],
+    "me_kvq_attn": [_p, _p, _i64, _i64, _p, _i, _p, _i, _p, _i64, _i64, _p, ctypes.c_size_t, _i, _i, _p, _i, _i, _p],
     "me_greedy_pick": [_p, _i, _i, _p, _i, _p, _i, _p],
     "me_sample_topk_topp": [_p, _i, _i, _p, _i, _p, _i, _f, _p, _p, _p, _p, _p, _i, _p],
     "me_sample_step": [_p, _i, _i, _p, _i, _p, _p, _p, _f, _f, _f, _i, _f, _p, _i, _p, _i, _p, _p, _i, _p],
@@ -83,6 +83,11 @@ class TnItem(ctypes.Structure):
 class DecLayer(ctypes.Structure):
     """struct me_dec_layer of include/midiemo.h (one layer's pointers for me_dec_token; the table lives in DEVICE memory)."""
     _fields_ = [(n, _p) for n in ("Wqkv", "bqkv", "Wo", "bo", "W1", "b1", "W2", "b2", "ln1_g", "ln1_b", "ln2_g", "ln2_b", "E", "kcache", "vcache")]
+
+
+class KVQCache(ctypes.Structure):
+    """struct me_kvq_cache of include/midiemo.h (a HOST struct; the tensors it points to belong to the caller)."""
+    _fields_ = [(n, _p) for n in ("kcodes", "kscale", "vcodes", "vscale")] + [(n, ctypes.c_int32) for n in ("B", "H", "dh", "blocks", "bits")]
 
 
 _lib = None

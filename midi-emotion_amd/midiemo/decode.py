@@ -210,8 +210,8 @@ class DecodeSession:
                 ops.dec_qkv(*(later or first), W["Wqkv"], W["bqkv"], self.xres[r0:r1], self.q[r0:r1], self.knew[r0:r1], self.vnew[r0:r1],
                             r1 - r0, d, H, dh, 1, 0, None, dt)
             c = self.kvq[i]
-            ops.kvq_write(k_rows, v_rows, c.k, c.k_scale, c.v, c.v_scale, c.bits, pos)
-            ops.kvq_attn(self.q.view(B, H, dh), c.k, c.k_scale, c.v, c.v_scale, None, c.bits, pos, W["E"], None, self.part, ns)
+            ops.kvq_write(c.ref, k_rows, v_rows, pos)
+            ops.kvq_attn(c.ref, self.q.view(B, H, dh), None, pos, W["E"], None, self.part, ns)
             for r0, r1 in chunks:
                 Mr = r1 - r0
                 ops.dec_proj_resid(self.part[r0 * H:r1 * H], ns, H, dh, None, W["Wo"], pv(p + "rga.fc.bias"), self.xres[r0:r1], self.s1[r0:r1],

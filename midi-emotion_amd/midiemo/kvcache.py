@@ -5,12 +5,15 @@ A row (one token, one head) of head_dim values is held as 4-bit e2m1 or 8-bit e4
 cut to bfloat16): 34 or 66 bytes at head_dim 64 against 128 in bf16.  The codes lie in the order in which the matrix instructions take
 them (include/midiemo.h describes it), 32 tokens to a block.  The decode step this serves: generate.py:92-122 of the
 reference, made incremental; the attention is music_multi.py:211-235 for one query row."""
+import contextlib
+
 import torch
 
 from . import ops
 
 HEAD_DIMS = (32, 48, 64)
 BLOCK = 32
+_HERE = contextlib.nullcontext()
 
 
 def _need(ok, what):
@@ -52,6 +55,9 @@ class QuantKVCache:
         self.max_len = k.shape[2] * BLOCK
         self.device = k.device
         self.nbytes = 2 * (k.numel() + 2 * k_scale.numel())
+        self._index = k.device.index
+        self._rows_strides = {}                 # host stride arrays by the strides they hold
+        self.ref = ops.kvq_cache(k, k_scale, v, v_scale, head_dim, bits) if k.device.type == "cuda" else None
 
     # -------------------------------------------------------------- checks
     def _here(self, *tensors):
@@ -75,8 +81,17 @@ class QuantKVCache:
         self._pos(pos, k.shape[1])
 
     def _on(self):
-        _need(self.device.type == "cuda", "it is on %s -- there is no CPU path" % self.device)
-        return torch.cuda.device(self.device)
+        """the cache's device as the current one (nothing to do where it is)"""
+        _need(self.ref is not None, "it is on %s -- there is no CPU path" % self.device)
+        return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
+
+    def _strides(self, k, v):
+        key = (k.stride(), v.stride())
+        if key not in self._rows_strides:
+            if len(self._rows_strides) > 64:
+                self._rows_strides.clear()
+            self._rows_strides[key] = ops.kvq_strides(k, v)
+        return self._rows_strides[key]
 
     # -------------------------------------------------------------- calls
     def write(self, k, v, pos, lens=None):
@@ -86,7 +101,7 @@ class QuantKVCache:
         if k.shape[1] == 0:
             return
         with self._on():
-            ops.kvq_write(k, v, self.k, self.k_scale, self.v, self.v_scale, self.bits, pos, lens)
+            ops.kvq_write(self.ref, k, v, pos, lens, self._strides(k, v))
 
     def read(self, pos, n, dtype=torch.float32, lens=None):
         """The rows at positions pos .. pos + n - 1 as (k, v) [B, n, H, head_dim] of `dtype`; rows from lens[b] on are zeros."""
@@ -95,7 +110,7 @@ class QuantKVCache:
         self._rows(k, v, pos, lens)
         with self._on():
             if k.shape[1] > 0:
-                ops.kvq_read(self.k, self.k_scale, self.v, self.v_scale, k, v, self.bits, pos, lens)
+                ops.kvq_read(self.ref, k, v, pos, lens, self._strides(k, v))
         return k, v
 
     def attend(self, q, pos, rel=None, key_pad=None, out=None, nsplit=0):
@@ -128,5 +143,5 @@ class QuantKVCache:
             ns = nsplit or ops.kvq_splits(self.batch, self.heads, tokens)
             # the records of this call: from the caching allocator, so calls on two streams or in two captured graphs never share them
             part = torch.empty(self.batch * self.heads * ns * (self.head_dim + 4), dtype=torch.float32, device=self.device) if ns > 1 else None
-            ops.kvq_attn(q, self.k, self.k_scale, self.v, self.v_scale, out, self.bits, pos, rel, key_pad, part, ns)
+            ops.kvq_attn(self.ref, q, out, pos, rel, key_pad, part, ns)
         return out

@@ -28,7 +28,8 @@ def _ptr(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream of the current device as torch's own wrapper has it, without building a Stream object (2 us of a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _code(dtype):
@@ -381,20 +382,28 @@ def _pos_args(pos):
 _I64x6 = ctypes.c_int64 * 6
 
 
-def kvq_write(k, v, kcodes, kscale, vcodes, vscale, bits, pos, lens=None):
+def kvq_cache(kcodes, kscale, vcodes, vscale, dh, bits):
+    """host descriptor of a quantised cache (struct me_kvq_cache) for the calls below; the caller keeps the tensors"""
+    return ctypes.byref(_lib.KVQCache(_ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale), kcodes.shape[0], kcodes.shape[1], int(dh), kcodes.shape[2], int(bits)))
+
+
+def kvq_strides(k, v):
+    """host array of the six strides of rows k, v [B, n, H, dh]"""
+    return _I64x6(*k.stride()[:3], *v.stride()[:3])
+
+
+def kvq_write(cache, k, v, pos, lens=None, strides=None):
     """quantise the rows k, v [B, n, H, dh] (any strides, dh contiguous) into the cache at positions pos .. (me_kvq_write)."""
-    B, n, H, dh = k.shape
     t, t_dev, ld_t = _pos_args(pos)
-    check(lib().me_kvq_write(_ptr(k), _ptr(v), _I64x6(*k.stride()[:3], *v.stride()[:3]), _ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale),
-                             B, n, H, dh, kcodes.shape[2], int(bits), t, t_dev, ld_t, _ptr(lens), _code(k.dtype), _stream()), "me_kvq_write")
+    check(lib().me_kvq_write(cache, _ptr(k), _ptr(v), strides or kvq_strides(k, v), k.shape[1], t, t_dev, ld_t, _ptr(lens), _code(k.dtype),
+                             _stream()), "me_kvq_write")
 
 
-def kvq_read(kcodes, kscale, vcodes, vscale, k, v, bits, pos, lens=None):
+def kvq_read(cache, k, v, pos, lens=None, strides=None):
     """the rows at positions pos .. pos + n - 1 into k, v [B, n, H, dh] (me_kvq_read); rows from lens[b] on become zeros."""
-    B, n, H, dh = k.shape
     t, t_dev, ld_t = _pos_args(pos)
-    check(lib().me_kvq_read(_ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale), _ptr(k), _ptr(v), _I64x6(*k.stride()[:3], *v.stride()[:3]),
-                            B, n, H, dh, kcodes.shape[2], int(bits), t, t_dev, ld_t, _ptr(lens), _code(k.dtype), _stream()), "me_kvq_read")
+    check(lib().me_kvq_read(cache, _ptr(k), _ptr(v), strides or kvq_strides(k, v), k.shape[1], t, t_dev, ld_t, _ptr(lens), _code(k.dtype),
+                            _stream()), "me_kvq_read")
 
 
 def kvq_splits(B, H, tokens):
@@ -402,17 +411,17 @@ def kvq_splits(B, H, tokens):
     return int(lib().me_kvq_splits(int(B), int(H), int(tokens)))
 
 
-def kvq_attn(q, kcodes, kscale, vcodes, vscale, out, bits, pos, E=None, key_pad=None, part=None, nsplit=1):
+def kvq_attn(cache, q, out, pos, E=None, key_pad=None, part=None, nsplit=1):
     """attention of one query per (sequence, head), q / out [B, H, dh], against the cached keys 0 .. pos (me_kvq_attn).
     part: uninitialised f32 buffer of workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh) bytes where nsplit > 1; out = None
     leaves the partial records in it (the form me_dec_proj_resid reads)."""
-    B, H, dh = q.shape
     t, t_dev, ld_t = _pos_args(pos)
-    check(lib().me_kvq_attn(_ptr(q), q.stride(0), q.stride(1), _ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale), _ptr(E),
-                            E.shape[0] if E is not None else 0, _ptr(key_pad), key_pad.stride(0) if key_pad is not None else 0, _ptr(out),
-                            out.stride(0) if out is not None else 0, out.stride(1) if out is not None else 0, _ptr(part),
-                            part.numel() * part.element_size() if part is not None else 0, int(nsplit), B, H, dh, kcodes.shape[2], int(bits), t,
-                            t_dev, ld_t, _code(q.dtype), _stream()), "me_kvq_attn")
+    qb, qh, _ = q.stride()
+    ob, oh, _ = out.stride() if out is not None else (0, 0, 0)
+    check(lib().me_kvq_attn(cache, _ptr(q), qb, qh, _ptr(E), E.shape[0] if E is not None else 0, _ptr(key_pad),
+                            key_pad.shape[1] if key_pad is not None else 0, _ptr(out), ob, oh, _ptr(part),
+                            part.numel() * part.element_size() if part is not None else 0, nsplit, t, t_dev, ld_t, _code(q.dtype), _stream()),
+          "me_kvq_attn")
 
 
 def sample_topk_topp(logits, V, special, temp, top_k, top_p, u, out_ids, n_choices=None, dbg_p=None, dbg_i=None):

@@ -80,13 +80,17 @@ def test_refusals_of_the_c_abi():
     P = 4096                                                           # never touched: the call is refused first
     six = (ctypes.c_int64 * 6)(*[64] * 6)
 
-    def write(k=P, kc=P, strides=six, B=1, n=1, H=1, dh=64, blocks=1, bits=4, t=0, t_dev=None, ld_t=0, dtype=_lib.ME_BF16):
-        return lib.me_kvq_write(k, P, strides, kc, P, P, P, B, n, H, dh, blocks, bits, t, t_dev, ld_t, None, dtype, None)
+    def cache(kc=P, B=1, H=1, dh=64, blocks=1, bits=4, vs=P):
+        return ctypes.byref(_lib.KVQCache(kc, P, P, vs, B, H, dh, blocks, bits))
 
-    def attn(q=P, kc=P, E=None, M=0, pad=None, ld_pad=0, out=P, part=None, part_bytes=0, nsplit=1, B=1, H=1, dh=64, blocks=1, bits=4, t=0, ld_t=0, dtype=_lib.ME_BF16):
-        return lib.me_kvq_attn(q, 64, 64, kc, P, P, P, E, M, pad, ld_pad, out, 64, 64, part, part_bytes, nsplit, B, H, dh, blocks, bits, t, None, ld_t, dtype, None)
+    def write(k=P, strides=six, n=1, t=0, t_dev=None, ld_t=0, dtype=_lib.ME_BF16, c=True, **kw):
+        return lib.me_kvq_write(cache(**kw) if c else None, k, P, strides, n, t, t_dev, ld_t, None, dtype, None)
+
+    def attn(q=P, E=None, M=0, pad=None, ld_pad=0, out=P, part=None, part_bytes=0, nsplit=1, t=0, ld_t=0, dtype=_lib.ME_BF16, c=True, **kw):
+        return lib.me_kvq_attn(cache(**kw) if c else None, q, 64, 64, E, M, pad, ld_pad, out, 64, 64, part, part_bytes, nsplit, t, None, ld_t, dtype, None)
 
     NULL, SHAPE, TYPE, ALIGN, WS = -5, -2, -1, -3, -6
+    assert write(c=False) == NULL and write(vs=None) == NULL and attn(c=False) == NULL
     assert write(k=None) == NULL and write(strides=None) == NULL and write(kc=P + 4) == ALIGN and write(dtype=7) == TYPE
     for bad in (dict(dh=40), dict(bits=2), dict(t=32), dict(t=-1), dict(n=33), dict(n=-1), dict(ld_t=2), dict(H=70000), dict(B=70000), dict(blocks=1 << 26), dict(B=-1)):
         assert write(**bad) == SHAPE, bad
@@ -98,4 +102,4 @@ def test_refusals_of_the_c_abi():
     assert need == 4 * 68 * 4
     assert attn(nsplit=4) == WS and attn(nsplit=4, part=P, part_bytes=need - 1) == WS and attn(out=None, part=P, part_bytes=68 * 4 - 4) == WS
     assert attn(B=0) == 0
-    assert lib.me_kvq_splits(1, 8, 2048) == 16 and lib.me_kvq_splits(1, 8, 100) == 1 and lib.me_kvq_splits(10 ** 6, 8, 2048) == 1 and lib.me_kvq_splits(1, 1, 1 << 30) == 64
+    assert lib.me_kvq_splits(1, 8, 2048) == 1 and lib.me_kvq_splits(1, 8, 100) == 1 and lib.me_kvq_splits(10 ** 6, 8, 2048) == 1 and lib.me_kvq_splits(1, 1, 1 << 30) == 64
