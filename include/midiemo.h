@@ -470,7 +470,7 @@ int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
  *     out = sum_j softmax_j( (q.k_j + q.E[M-1-(t-j)]) / sqrt(dh) ) v_j   over keys j = 0 .. t that key_pad leaves (music_multi.py:211-235)
  *   E (T [M][dh] natural layout, 16-byte aligned; NULL: no relative term) needs M >= 32 * blocks.  key_pad: uint8 [B][ld_pad] or NULL,
  *   1 = masked; keys from ld_pad on are not masked.  A masked row's codes and scale are never used, whatever they hold.  No
- *   key left (t = -1, or all masked): zeros.  nsplit in 1 .. 64 key ranges (me_kvq_splits gives a good number); with nsplit > 1
+ *   key left (t = -1, or all masked): zeros.  nsplit in 1 .. 64 key ranges (me_kvq_splits gives a good number; rel: with a relative table); with nsplit > 1
  *   `part` (me_workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh, dtype) bytes, 16-byte aligned, uninitialised, private to the
  *   call until it has run) holds the ranges' records and a second launch joins them in ascending order.  out = NULL: the records are the
  *   result, as me_dec_attn leaves them (nsplit <= 8: me_dec_proj_resid joins them; it takes a row without keys for NaN). */
@@ -482,7 +482,7 @@ int me_kvq_write(const me_kvq_cache* c, const void* k, const void* v, const int6
                  const int32_t* lens, int dtype, void* stream);
 int me_kvq_read(const me_kvq_cache* c, void* k, void* v, const int64_t* strides, int n, int t, const int32_t* t_dev, int ld_t, const int32_t* lens,
                 int dtype, void* stream);
-int me_kvq_splits(int B, int H, int tokens);
+int me_kvq_splits(int B, int H, int tokens, int rel);
 int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* E, int M, const uint8_t* key_pad, int ld_pad,
                 void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes, int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype,
                 void* stream);

@@ -380,6 +380,48 @@ template <int DH> ME_DEV int slot_dim(int r, int sg, int i) {
     return sg == 1 && (i >> 4) == half ? 32 + (i & 15) : -1;
 }
 
+// a row's operand (one of 16 rows, lane group g's share of the contraction) of the relative product q E^T in T
+template <typename T, int DH> struct EFrag {
+    static constexpr int N = (DH + 31) / 32;
+    typename V16<T>::x8 v[N];
+    ME_DEV void load(const T* p, int g) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            v[k] = (typename V16<T>::x8){0, 0, 0, 0, 0, 0, 0, 0};
+            if (32 * k + 8 * g < DH) v[k] = *reinterpret_cast<const typename V16<T>::x8*>(p + 32 * k + 8 * g);
+        }
+    }
+    ME_DEV void set(const float* p, int g) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = 32 * k + 8 * g < DH ? (T)p[32 * k + 8 * g + i] : (T)0.f;
+    }
+    ME_DEV static f32x4_t mma(const EFrag& x, const EFrag& y) {
+        f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if constexpr (__is_same(T, bf16_t)) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v[k], y.v[k], d, 0, 0, 0);
+            else d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.v[k], y.v[k], d, 0, 0, 0);
+        }
+        return d;
+    }
+};
+template <int DH> struct EFrag<float, DH> {                   // group g takes a quarter of the row
+    f32x4_t v[DH / 16];
+    ME_DEV void load(const float* p, int g) {
+#pragma unroll
+        for (int k = 0; k < DH / 16; ++k) v[k] = *reinterpret_cast<const f32x4_t*>(p + g * (DH / 4) + 4 * k);
+    }
+    ME_DEV void set(const float* p, int g) { load(p, g); }
+    ME_DEV static f32x4_t mma(const EFrag& x, const EFrag& y) {
+        f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < DH / 4; ++k) d = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[k >> 2][k & 3], y.v[k >> 2][k & 3], d, 0, 0, 0);
+        return d;
+    }
+};
+
 template <typename T, int BITS, int DH, bool REL>
 __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) {
     constexpr bool WIDE = sizeof(T) == 4;
@@ -388,7 +430,7 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
     constexpr int NS = BITS == 4 && WIDE ? 2 : 1;             // operand sets of four rows
     constexpr int PR = PROW<BITS>;
     constexpr float LOG2E = 1.4426950408889634f;
-    __shared__ float qs[HG][DH];
+    __shared__ __attribute__((aligned(16))) float qs[HG][DH];
     __shared__ __attribute__((aligned(16))) uint8_t parts[WAVES][NP * PR];
     __shared__ float rel[REL ? RELS : 1];
     __shared__ float jm[WAVES], jl[WAVES], jo[WAVES][DH];     // key ranges of a head meet here
@@ -477,35 +519,31 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
     for (int u = 0; u < DH / 16; ++u) acc[u] = 0.f;
     const float cs = a.scale * LOG2E, cq = cs * qinv;
 
+    EFrag<T, DH> eq;                                          // row c: the query of the block's head c (rows past the last repeat it)
+    if constexpr (REL) eq.set(qs[min(c, nh - 1)], g);
     const int stretch = REL ? RELS / hpb : max(j1 - j0, 1);   // a multiple of kw tiles
     for (int c0 = j0; c0 < j1; c0 += stretch) {
         const int c1 = min(c0 + stretch, j1);
         if constexpr (REL) {
             const int t = n - 1;
             __syncthreads();                                  // the last stretch has been read
-            for (int kt = wid * 16; kt < c1 - c0; kt += nw * 16) {
-                const int row = a.M - 1 - t + min(c0 + kt + c, t);
-                const T* er = reinterpret_cast<const T*>(a.E) + (size_t)row * DH;
-                f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (WIDE) {
+            constexpr int U = 4;                              // key groups of 16 in flight per wave
+            for (int k0 = wid * 16; k0 < c1 - c0; k0 += nw * 16 * U) {
+                EFrag<T, DH> e[U];
 #pragma unroll
-                    for (int k = 0; k < DH; k += 4) d = __builtin_amdgcn_mfma_f32_16x16x4f32(qs[min(c, nh - 1)][k + g], er[k + g], d, 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < DH; k += 32) {
-                        typename V16<T>::x8 x = {0, 0, 0, 0, 0, 0, 0, 0}, y = x;
-                        const int d0 = k + 8 * g;
-                        if (d0 < DH) {
-                            y = *reinterpret_cast<const typename V16<T>::x8*>(er + d0);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = (T)qs[min(c, nh - 1)][d0 + e];
-                        }
-                        if constexpr (__is_same(T, bf16_t)) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, d, 0, 0, 0);
-                        else d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, d, 0, 0, 0);
-                    }
+                for (int u = 0; u < U; ++u) {
+                    const int row = a.M - 1 - t + min(c0 + k0 + u * nw * 16 + c, t);
+                    e[u].load(reinterpret_cast<const T*>(a.E) + (size_t)row * DH, g);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (4 * g + i < nh) rel[(4 * g + i) * stretch + kt + c] = d[i];
+                for (int u = 0; u < U; ++u) {
+                    const int kt = k0 + u * nw * 16;
+                    const f32x4_t d = EFrag<T, DH>::mma(eq, e[u]);
+                    if (kt < c1 - c0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) if (4 * g + i < nh) rel[(4 * g + i) * stretch + kt + c] = d[i];
+                    }
+                }
             }
             __syncthreads();
         }
@@ -664,14 +702,26 @@ template <typename T, int DH>
 __global__ __launch_bounds__(256) void kvq_join_kernel(const float* __restrict__ part, int nsplit, int BH, int H, T* __restrict__ out, int64_t sob, int64_t soh) {
     const int lane = threadIdx.x & 63, bh = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (bh >= BH) return;
-    const float* rec = part + (size_t)bh * nsplit * ME_DEC_PART_REC(DH);
-    const float2 ml = lane < nsplit ? *reinterpret_cast<const float2*>(rec + (size_t)lane * ME_DEC_PART_REC(DH)) : make_float2(-INFINITY, 0.f);
+    constexpr int REC = ME_DEC_PART_REC(DH), U = 8;
+    const float* rec = part + (size_t)bh * nsplit * REC;
+    const float2 ml = lane < nsplit ? *reinterpret_cast<const float2*>(rec + (size_t)lane * REC) : make_float2(-INFINITY, 0.f);
+    const float* po = rec + 4 + min(lane, DH - 1);
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = po[(size_t)min(u, nsplit - 1) * REC];      // requested with the maxima: one round trip up to 8 splits
     const float mx = wave_max(ml.x), ms = mx == -INFINITY ? 0.f : mx;
     const float w = lane < nsplit ? exp2f(ml.x - ms) : 0.f, l = wave_sum(w * ml.y);
     float o = 0.f;
-    for (int s = 0; s < nsplit; ++s) {
-        const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s));
-        if (lane < DH) o = fmaf(ws, rec[(size_t)s * ME_DEC_PART_REC(DH) + 4 + lane], o);
+    for (int s0 = 0; s0 < nsplit; s0 += U) {
+        float nx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) nx[u] = s0 + U < nsplit ? po[(size_t)min(s0 + U + u, nsplit - 1) * REC] : 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(s0 + u, 63)));
+            if (s0 + u < nsplit) o = fmaf(ws, v[u], o);
+            v[u] = nx[u];
+        }
     }
     if (lane < DH) out[(int64_t)(bh / H) * sob + (int64_t)(bh % H) * soh + lane] = ET<T>::from_f(l == 0.f ? 0.f : o / l);
 }
@@ -756,12 +806,18 @@ int me_kvq_read(const me_kvq_cache* c, void* k, void* v, const int64_t* strides,
     return rows_call(false, c, k, v, strides, n, t, t_dev, ld_t, lens, dtype, (hipStream_t)stream);
 }
 
-// A second launch joins the splits, so a cache is only cut where its (sequence, head) pairs leave most of the chip idle and every wave
-// keeps two tiles.
-int me_kvq_splits(int B, int H, int tokens) {
+// How the keys are cut.  2048 waves (8 per CU) are enough to keep the memory busy; a row (sequence, head) that has fewer is cut into
+// ranges: first inside the block (ranges meet in LDS), then over blocks, whose records a second launch joins (2 .. 3 us).  The
+// relative products want blocks of many heads (a stretch's rows of E are read once per block) but 256 blocks, one per CU, come first.
+// Measured, us per call, 4 bits, dh 64, one block per row and all ranges in it -> as chosen here:
+//   relative table: 1 x 8 rows of 2048 keys 13.5 -> 7.4, 4 x 8: 14.5 -> 8.0, 16 x 8: 15.6 -> 11.2, 64 x 8: 34.0 -> 20.4; up to 512 keys
+//   one launch is faster (4 x 8 of 512: 6.5, four splits 7.0);  none: 1 x 8 of 16384 keys 8 splits 9.2, 16: 8.5; 16 x 8 of 4096: two splits 12.6, none 12.0.
+int me_kvq_splits(int B, int H, int tokens, int rel) {
     if (B <= 0 || H <= 0 || tokens <= 0) return 1;
     const int64_t rows = (int64_t)B * H, tiles = ((int64_t)tokens + TK - 1) / TK;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(256 / rows, tiles / (2 * WAVES)), 64));
+    if (rel) return tiles <= 4 || rows > 512 ? 1 : (int)std::min<int64_t>(std::min<int64_t>(2048 / rows, tiles), 64);
+    const int64_t ns = std::min<int64_t>(std::min<int64_t>(2048 / (rows * WAVES), tiles / WAVES), 64);
+    return ns > 2 ? (int)ns : 1;
 }
 
 int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* E, int M, const uint8_t* key_pad, int ld_pad,
@@ -777,12 +833,11 @@ int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq
     if (c->B == 0 || c->H == 0) return ME_OK;
     const bool split = nsplit > 1 || !out;                    // out == NULL: the partial records are the result (me_dec_proj_resid joins them)
     if (split && (!part || part_bytes < (size_t)c->B * c->H * nsplit * ME_DEC_PART_REC(c->dh) * 4)) return ME_ERR_WORKSPACE;
-    // heads per block: the relative products of a stretch of keys are shared by a block's heads, so as many as leave two blocks per CU;
-    // key ranges per head: what is left of the block's 8 waves, if there are tiles for them
+    // key ranges inside the block up to 2048 waves, then heads into the block while 256 blocks are left (see me_kvq_splits)
     int hpb = 1, kw = 1;
-    const int64_t tiles = ((((t_dev ? (int64_t)c->blocks * KB : (int64_t)t + 1) + nsplit - 1) / nsplit) + TK - 1) / TK;
-    while (E && hpb < HG && 2 * hpb <= c->H && (int64_t)nsplit * c->B * ((c->H + 2 * hpb - 1) / (2 * hpb)) >= 512) hpb *= 2;
-    while (hpb * kw < WAVES && kw < tiles) kw *= 2;
+    const int64_t tiles = ((((t_dev ? (int64_t)c->blocks * KB : (int64_t)t + 1) + nsplit - 1) / nsplit) + TK - 1) / TK, cut = (int64_t)nsplit * c->B;
+    while (kw < WAVES && kw < tiles && cut * c->H * kw <= 1024) kw *= 2;
+    while (E && hpb * kw < WAVES && hpb < HG && 2 * hpb <= c->H && cut * ((c->H + 2 * hpb - 1) / (2 * hpb)) >= 256) hpb *= 2;
     AttnArgs a = {q, ldq_b, ldq_h, (const uint8_t*)c->kcodes, (const u16*)c->kscale, (const uint8_t*)c->vcodes, (const u16*)c->vscale, E, M, key_pad, ld_pad,
                   out, ldo_b, ldo_h, split ? part : nullptr, nsplit, c->H, c->blocks, t, ld_t, hpb, kw, t_dev, 1.f / sqrtf((float)c->dh), out ? 1.f : 0.6931471805599453f};
     if (dtype == ME_F32) attn_call<float>(a, c->B, c->dh, c->bits, split && out, (hipStream_t)stream);

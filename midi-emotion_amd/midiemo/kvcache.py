@@ -140,7 +140,7 @@ class QuantKVCache:
             tokens = max(int(pos) + 1, 1)
         _need(0 <= nsplit <= 64, "nsplit must be 0..64")
         with self._on():
-            ns = nsplit or ops.kvq_splits(self.batch, self.heads, tokens)
+            ns = nsplit or ops.kvq_splits(self.batch, self.heads, tokens, rel is not None)
             # the records of this call: from the caching allocator, so calls on two streams or in two captured graphs never share them
             part = torch.empty(self.batch * self.heads * ns * (self.head_dim + 4), dtype=torch.float32, device=self.device) if ns > 1 else None
             ops.kvq_attn(self.ref, q, out, pos, rel, key_pad, part, ns)

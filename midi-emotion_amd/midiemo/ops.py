@@ -406,9 +406,9 @@ def kvq_read(cache, k, v, pos, lens=None, strides=None):
                             _stream()), "me_kvq_read")
 
 
-def kvq_splits(B, H, tokens):
+def kvq_splits(B, H, tokens, rel=False):
     """key ranges me_kvq_attn should cut a cache of that many tokens into (1 .. 64)"""
-    return int(lib().me_kvq_splits(int(B), int(H), int(tokens)))
+    return int(lib().me_kvq_splits(int(B), int(H), int(tokens), int(bool(rel))))
 
 
 def kvq_attn(cache, q, out, pos, E=None, key_pad=None, part=None, nsplit=1):

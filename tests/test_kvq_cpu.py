@@ -102,4 +102,7 @@ def test_refusals_of_the_c_abi():
     assert need == 4 * 68 * 4
     assert attn(nsplit=4) == WS and attn(nsplit=4, part=P, part_bytes=need - 1) == WS and attn(out=None, part=P, part_bytes=68 * 4 - 4) == WS
     assert attn(B=0) == 0
-    assert lib.me_kvq_splits(1, 8, 2048) == 1 and lib.me_kvq_splits(1, 8, 100) == 1 and lib.me_kvq_splits(10 ** 6, 8, 2048) == 1 and lib.me_kvq_splits(1, 1, 1 << 30) == 64
+    for rel in (0, 1):
+        for b, h, n in ((1, 8, 1), (1, 8, 2048), (4, 8, 2048), (64, 16, 1999), (1, 1, 1 << 30), (10 ** 6, 8, 2048), (0, 1, 1)):
+            assert 1 <= lib.me_kvq_splits(b, h, n, rel) <= 64
+    assert lib.me_kvq_splits(4, 8, 2048, 1) == 16 and lib.me_kvq_splits(4, 8, 2048, 0) == 1 and lib.me_kvq_splits(1, 1, 1 << 30, 0) == 64
