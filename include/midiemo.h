@@ -486,6 +486,12 @@ int me_kvq_splits(int B, int H, int tokens, int rel);
 int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* E, int M, const uint8_t* key_pad, int ld_pad,
                 void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes, int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype,
                 void* stream);
+/* A decode step's write and attention in one launch: the rows k, v (T [B][H][dh], strides ldn_* for both, 16-byte aligned throughout) are
+ * quantised into position t (per sequence) as me_kvq_write does it, and the query attends to keys 0 .. t, the new one through its held
+ * (quantised) values.  Same results as the two calls up to f32 summation order.  A position outside the cache is not written. */
+int me_kvq_append_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* k, const void* v, int64_t ldn_b, int64_t ldn_h,
+                       const void* E, int M, const uint8_t* key_pad, int ld_pad, void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes,
+                       int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype, void* stream);
 
 /* Greedy pick for generate(top_k=1): logits f32 [B, ld]; NaN -> 0, ids in
  * special[0..n_special) -> -inf, argmax -> out_ids[B] (generate.py:122-136,166-183). */

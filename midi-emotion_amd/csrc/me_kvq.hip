@@ -300,6 +300,7 @@ struct AttnArgs {
     const uint8_t* pad; int ld_pad;
     void* out; int64_t sob, soh;
     float* part; int nsplit;
+    const void* kn; const void* vn; int64_t snb, snh;         // the rows of position t itself, still to be cached (or NULL)
     int H, blocks, t, ld_t, hpb, kw;
     const int32_t* t_dev;
     float scale;
@@ -439,9 +440,10 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
     const int hpb = a.hpb, kw = a.kw, hw = wid / kw, wk = wid % kw;
     const int split = blockIdx.x, b = blockIdx.z, h0 = blockIdx.y * hpb, nh = min(hpb, a.H - h0);
     const int hh = min(hw, nh - 1), h = h0 + hh;              // waves past the last head repeat it and store nothing
-    int n = min(pos_of(a.t, a.t_dev, a.ld_t, b), a.blocks * KB - 1) + 1;
-    if (REL) n = min(n, a.M);
-    n = max(n, 0);
+    const int t = pos_of(a.t, a.t_dev, a.ld_t, b);
+    const bool fresh = a.kn && t >= 0 && t < a.blocks * KB;   // position t comes with the call; the keys before it are in the cache
+    const int n = fresh ? t : max(min(t, a.blocks * KB - 1) + 1, 0);
+    const int last = fresh ? t : n - 1;                       // the query's position
     const int per = ((n + a.nsplit - 1) / a.nsplit + TK - 1) / TK * TK;
     const int j0 = (int)min((int64_t)split * per, (int64_t)n), j1 = (int)min((int64_t)j0 + per, (int64_t)n);
     const size_t bh = (size_t)b * a.H + h;
@@ -519,20 +521,79 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
     for (int u = 0; u < DH / 16; ++u) acc[u] = 0.f;
     const float cs = a.scale * LOG2E, cq = cs * qinv;
 
+    // ---- position t itself: quantised into the cache by the first range's wave (lanes 0..7 K, 8..15 V: 8 values each), which starts its
+    //      softmax with it, from the held values in 32 bits -- the cache is not read where this launch writes it
+    if (fresh && split == 0 && wk == 0 && hw < nh) {
+        const int sub = lane & 7, d0 = sub * 8, tk = t & (KB - 1);
+        const bool isv = lane >= 8, on = lane < 16 && d0 < DH;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (on) load8<T, true>(x, reinterpret_cast<const T*>(isv ? a.vn : a.kn) + (int64_t)b * a.snb + (int64_t)h * a.snh + d0);
+        u16 sc;
+        uint32_t cd[2];
+        quantise8<BITS, WIDE>(x, sc, cd, on);
+        const size_t blk = (size_t)(t / KB) * Fmt<BITS, DH>::BLK;
+        if (on && !isv) {
+            uint32_t* p = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(kc) + blk + k_byte<BITS, DH>(tk, d0));
+            p[0] = cd[0];
+            if (BITS == 8) p[1] = cd[1];
+        }
+        if (on && isv) {
+            uint8_t* p = const_cast<uint8_t*>(vc) + blk + (BITS == 4 ? tk >> 1 : (tk >> 4) * (DH * 16) + (tk & 15)) + d0 * 16;
+            if (BITS == 4) {
+                uint32_t old[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) old[i] = p[16 * i];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t cc = (cd[0] >> (4 * i)) & 15u;
+                    p[16 * i] = (uint8_t)(tk & 1 ? (old[i] & 15u) | (cc << 4) : (old[i] & 0xf0u) | cc);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[16 * i] = (uint8_t)(cd[i >> 2] >> (8 * (i & 3)));
+            }
+        }
+        if (lane == 0) const_cast<u16*>(ks)[t] = sc;
+        if (lane == 8) const_cast<u16*>(vs)[t] = sc;
+        expand8<BITS>(x, cd[0], cd[1], bf16_bits(sc));
+        float s = 0.f;
+        if (on && !isv) {
+            float e[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if constexpr (REL) load8<T, true>(e, reinterpret_cast<const T*>(a.E) + (size_t)(a.M - 1) * DH + d0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s = fmaf(qs[hh][d0 + i], x[i] + e[i], s);
+        }
+        if (on && isv) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) jo[wid][d0 + i] = x[i];
+        }
+        s = wave_sum(s) * cs;
+        lds_order();
+        if (!(pad && t < a.ld_pad && pad[t]) && s != -INFINITY) {
+            const float one = __builtin_amdgcn_exp2f(s - s);  // 1, or NaN where the logit is none
+            m = s;
+            lsum = lane == 0 ? one : 0.f;
+#pragma unroll
+            for (int u = 0; u < DH / 16; ++u) acc[u] = one * jo[wid][16 * u + (lane & 15)];
+        }
+        lds_order();
+    }
+
     EFrag<T, DH> eq;                                          // row c: the query of the block's head c (rows past the last repeat it)
     if constexpr (REL) eq.set(qs[min(c, nh - 1)], g);
     const int stretch = REL ? RELS / hpb : max(j1 - j0, 1);   // a multiple of kw tiles
     for (int c0 = j0; c0 < j1; c0 += stretch) {
         const int c1 = min(c0 + stretch, j1);
         if constexpr (REL) {
-            const int t = n - 1;
             __syncthreads();                                  // the last stretch has been read
             constexpr int U = 4;                              // key groups of 16 in flight per wave
             for (int k0 = wid * 16; k0 < c1 - c0; k0 += nw * 16 * U) {
                 EFrag<T, DH> e[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int row = a.M - 1 - t + min(c0 + k0 + u * nw * 16 + c, t);
+                    const int row = a.M - 1 - last + min(c0 + k0 + u * nw * 16 + c, last);
                     e[u].load(reinterpret_cast<const T*>(a.E) + (size_t)row * DH, g);
                 }
 #pragma unroll
@@ -820,16 +881,17 @@ int me_kvq_splits(int B, int H, int tokens, int rel) {
     return ns > 2 ? (int)ns : 1;
 }
 
-int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* E, int M, const uint8_t* key_pad, int ld_pad,
-                void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes, int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype,
-                void* stream) {
+static int attn_entry(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* kn, const void* vn, int64_t ldn_b, int64_t ldn_h,
+                      const void* E, int M, const uint8_t* key_pad, int ld_pad, void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes,
+                      int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype, void* stream) {
     me_clear_error();
     if (!q || (!out && !part)) return ME_ERR_NULL;
     if (int rc = cache_status(c)) return rc;
     if (dtype != ME_F32 && dtype != ME_BF16 && dtype != ME_F16) return ME_ERR_BAD_DTYPE;
     if (nsplit < 1 || nsplit > 64 || (ld_t != 0 && ld_t != 1) || (!t_dev && (t < -1 || t >= c->blocks * KB)) || (E && M < c->blocks * KB) ||
         (key_pad && ld_pad < 0)) return ME_ERR_BAD_SHAPE;
-    if ((E && !aligned16(E)) || (part && !aligned16(part))) return ME_ERR_ALIGNMENT;
+    const int es = dtype == ME_F32 ? 4 : 2;
+    if ((E && !aligned16(E)) || (part && !aligned16(part)) || (kn && (!aligned16(kn) || !aligned16(vn) || (ldn_b * es) % 16 || (ldn_h * es) % 16))) return ME_ERR_ALIGNMENT;
     if (c->B == 0 || c->H == 0) return ME_OK;
     const bool split = nsplit > 1 || !out;                    // out == NULL: the partial records are the result (me_dec_proj_resid joins them)
     if (split && (!part || part_bytes < (size_t)c->B * c->H * nsplit * ME_DEC_PART_REC(c->dh) * 4)) return ME_ERR_WORKSPACE;
@@ -839,11 +901,25 @@ int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq
     while (kw < WAVES && kw < tiles && cut * c->H * kw <= 1024) kw *= 2;
     while (E && hpb * kw < WAVES && hpb < HG && 2 * hpb <= c->H && cut * ((c->H + 2 * hpb - 1) / (2 * hpb)) >= 256) hpb *= 2;
     AttnArgs a = {q, ldq_b, ldq_h, (const uint8_t*)c->kcodes, (const u16*)c->kscale, (const uint8_t*)c->vcodes, (const u16*)c->vscale, E, M, key_pad, ld_pad,
-                  out, ldo_b, ldo_h, split ? part : nullptr, nsplit, c->H, c->blocks, t, ld_t, hpb, kw, t_dev, 1.f / sqrtf((float)c->dh), out ? 1.f : 0.6931471805599453f};
+                  out, ldo_b, ldo_h, split ? part : nullptr, nsplit, kn, vn, ldn_b, ldn_h, c->H, c->blocks, t, ld_t, hpb, kw, t_dev, 1.f / sqrtf((float)c->dh), out ? 1.f : 0.6931471805599453f};
     if (dtype == ME_F32) attn_call<float>(a, c->B, c->dh, c->bits, split && out, (hipStream_t)stream);
     else if (dtype == ME_BF16) attn_call<bf16_t>(a, c->B, c->dh, c->bits, split && out, (hipStream_t)stream);
     else attn_call<f16_t>(a, c->B, c->dh, c->bits, split && out, (hipStream_t)stream);
     return me_launch_status();
+}
+
+int me_kvq_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* E, int M, const uint8_t* key_pad, int ld_pad,
+                void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes, int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype,
+                void* stream) {
+    return attn_entry(c, q, ldq_b, ldq_h, nullptr, nullptr, 0, 0, E, M, key_pad, ld_pad, out, ldo_b, ldo_h, part, part_bytes, nsplit, t, t_dev, ld_t, dtype, stream);
+}
+
+int me_kvq_append_attn(const me_kvq_cache* c, const void* q, int64_t ldq_b, int64_t ldq_h, const void* k, const void* v, int64_t ldn_b, int64_t ldn_h,
+                       const void* E, int M, const uint8_t* key_pad, int ld_pad, void* out, int64_t ldo_b, int64_t ldo_h, float* part, size_t part_bytes,
+                       int nsplit, int t, const int32_t* t_dev, int ld_t, int dtype, void* stream) {
+    if (!k || !v) return ME_ERR_NULL;
+    if (!t_dev && t < 0) return ME_ERR_BAD_SHAPE;
+    return attn_entry(c, q, ldq_b, ldq_h, k, v, ldn_b, ldn_h, E, M, key_pad, ld_pad, out, ldo_b, ldo_h, part, part_bytes, nsplit, t, t_dev, ld_t, dtype, stream);
 }
 
 }  // extern "C"

@@ -64,6 +64,7 @@ SIGNATURES = {
     "me_kvq_read": [_p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _p],
     "me_kvq_splits": [_i, _i, _i, _i],
     "me_kvq_attn": [_p, _p, _i64, _i64, _p, _i, _p, _i, _p, _i64, _i64, _p, ctypes.c_size_t, _i, _i, _p, _i, _i, _p],
+    "me_kvq_append_attn": [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i, _p, _i, _p, _i64, _i64, _p, ctypes.c_size_t, _i, _i, _p, _i, _i, _p],
     "me_greedy_pick": [_p, _i, _i, _p, _i, _p, _i, _p],
     "me_sample_topk_topp": [_p, _i, _i, _p, _i, _p, _i, _f, _p, _p, _p, _p, _p, _i, _p],
     "me_sample_step": [_p, _i, _i, _p, _i, _p, _p, _p, _f, _f, _f, _i, _f, _p, _i, _p, _i, _p, _p, _i, _p],

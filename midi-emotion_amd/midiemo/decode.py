@@ -24,7 +24,7 @@ embedding; in both cases the caller falls back to full recompute (exact
 reference semantics) -- see generate.py.
 
 `kv_bits` = 4 or 8 holds the caches quantised (kvcache.QuantKVCache: 34 / 66 bytes per row of 64 values instead of 128 in bf16): the
-projection leaves the new rows in a staging row, me_kvq_write quantises them into place and me_kvq_attn reads the codes as they lie;
+projection leaves the new rows in a staging row, me_kvq_append_attn quantises them into place and reads the older codes as they lie;
 its partial records are the ones me_dec_proj_resid joins, everything else of the step is unchanged.
 """
 import os
@@ -57,7 +57,7 @@ class DecodeSession:
         self.kv_bits = kv_bits
         if kv_bits:
             self.kvq = [QuantKVCache(B, H, m.max_seq, dh, kv_bits, dev) for _ in range(m.num_layer)]
-            self.knew, self.vnew = e(B, H, 1, dh), e(B, H, 1, dh)          # a step's rows before they are quantised
+            self.knew, self.vnew = e(B, H, dh), e(B, H, dh)                # a step's rows before they are quantised
         else:
             self.kc = [torch.zeros(B, H, m.max_seq, dh, dtype=dt, device=dev) for _ in range(m.num_layer)]
             self.vc = [torch.zeros(B, H, m.max_seq, dh, dtype=dt, device=dev) for _ in range(m.num_layer)]
@@ -201,7 +201,6 @@ class DecodeSession:
             ops.embed_fwd(x_hi, tokens, cond if cw is not None else None, pv("embedding.weight"), cw, cb, None, None, m._pe if self._pos_dev is not None else m._pe[t:],
                           ops.ME_COND_CONCAT if cw is not None else ops.ME_COND_NONE, B, 1, d, m.d_condition if cw is not None else 0, 0.0, 0,
                           pos_dev=self._pos_dev, out_lo=x_lo)
-        k_rows, v_rows = self.knew.transpose(1, 2), self.vnew.transpose(1, 2)
         for i in range(m.num_layer):
             W, p, pp = m._prep["layers"][i], f"enc_layers.{i}.", f"enc_layers.{i - 1}."
             for r0, r1 in chunks:
@@ -210,8 +209,7 @@ class DecodeSession:
                 ops.dec_qkv(*(later or first), W["Wqkv"], W["bqkv"], self.xres[r0:r1], self.q[r0:r1], self.knew[r0:r1], self.vnew[r0:r1],
                             r1 - r0, d, H, dh, 1, 0, None, dt)
             c = self.kvq[i]
-            ops.kvq_write(c.ref, k_rows, v_rows, pos)
-            ops.kvq_attn(c.ref, self.q.view(B, H, dh), None, pos, W["E"], None, self.part, ns)
+            ops.kvq_append_attn(c.ref, self.q.view(B, H, dh), self.knew, self.vnew, None, pos, W["E"], None, self.part, ns)
             for r0, r1 in chunks:
                 Mr = r1 - r0
                 ops.dec_proj_resid(self.part[r0 * H:r1 * H], ns, H, dh, None, W["Wo"], pv(p + "rga.fc.bias"), self.xres[r0:r1], self.s1[r0:r1],
@@ -235,7 +233,7 @@ class DecodeSession:
             return 2                                                # the token + pick / commit
         if self.kv_bits:
             chunks = -(-self.B // ROWS)
-            return (2 + 4 * chunks) * self.m.num_layer + 1 + chunks + 1     # + embedding, head, pick / commit
+            return (1 + 4 * chunks) * self.m.num_layer + 1 + chunks + 1     # + embedding, head, pick / commit
         return (4 if self.fused else 5) * self.m.num_layer + 2     # + head, + pick / commit
 
     def check_token_status(self):

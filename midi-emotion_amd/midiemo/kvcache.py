@@ -113,7 +113,17 @@ class QuantKVCache:
                 ops.kvq_read(self.ref, k, v, pos, lens, self._strides(k, v))
         return k, v
 
-    def attend(self, q, pos, rel=None, key_pad=None, out=None, nsplit=0):
+    def append_attend(self, q, k, v, pos, rel=None, key_pad=None, out=None, nsplit=0):
+        """A decode step in one launch: write the rows k, v [B, H, head_dim] at pos, then attend to the keys 0 .. pos.  k and v are of q's type with
+        equal strides, their rows 16-byte aligned."""
+        for x in (k, v):
+            _need(x.shape == (self.batch, self.heads, self.head_dim) and x.dtype == q.dtype and x.stride() == k.stride() and x.stride(2) == 1,
+                  "new rows must be [%d, %d, %d] of q's type with equal strides and the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
+        self._here(k, v)
+        _need(isinstance(pos, torch.Tensor) or pos >= 0, "position %r has no row to write" % (pos,))
+        return self.attend(q, pos, rel, key_pad, out, nsplit, (k, v))
+
+    def attend(self, q, pos, rel=None, key_pad=None, out=None, nsplit=0, _rows=None):
         """softmax((q.k_j + q.rel[M-1-(pos-j)]) / sqrt(head_dim)) v over the cached keys j = 0 .. pos (pos = -1: none).
 
         q [B, H, head_dim]; rel [M, head_dim] of q's type with M >= max_len (the model's relative table) or None; key_pad uint8 / bool
@@ -143,5 +153,8 @@ class QuantKVCache:
             ns = nsplit or ops.kvq_splits(self.batch, self.heads, tokens, rel is not None)
             # the records of this call: from the caching allocator, so calls on two streams or in two captured graphs never share them
             part = torch.empty(self.batch * self.heads * ns * (self.head_dim + 4), dtype=torch.float32, device=self.device) if ns > 1 else None
-            ops.kvq_attn(self.ref, q, out, pos, rel, key_pad, part, ns)
+            if _rows:
+                ops.kvq_append_attn(self.ref, q, _rows[0], _rows[1], out, pos, rel, key_pad, part, ns)
+            else:
+                ops.kvq_attn(self.ref, q, out, pos, rel, key_pad, part, ns)
         return out

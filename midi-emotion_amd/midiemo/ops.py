@@ -424,6 +424,18 @@ def kvq_attn(cache, q, out, pos, E=None, key_pad=None, part=None, nsplit=1):
           "me_kvq_attn")
 
 
+def kvq_append_attn(cache, q, k, v, out, pos, E=None, key_pad=None, part=None, nsplit=1):
+    """kvq_write of the rows k, v [B, H, dh] (equal strides) at pos and kvq_attn over the keys 0 .. pos in one launch (me_kvq_append_attn)."""
+    t, t_dev, ld_t = _pos_args(pos)
+    qb, qh, _ = q.stride()
+    nb, nh, _ = k.stride()
+    ob, oh, _ = out.stride() if out is not None else (0, 0, 0)
+    check(lib().me_kvq_append_attn(cache, _ptr(q), qb, qh, _ptr(k), _ptr(v), nb, nh, _ptr(E), E.shape[0] if E is not None else 0, _ptr(key_pad),
+                                   key_pad.shape[1] if key_pad is not None else 0, _ptr(out), ob, oh, _ptr(part),
+                                   part.numel() * part.element_size() if part is not None else 0, nsplit, t, t_dev, ld_t, _code(q.dtype), _stream()),
+          "me_kvq_append_attn")
+
+
 def sample_topk_topp(logits, V, special, temp, top_k, top_p, u, out_ids, n_choices=None, dbg_p=None, dbg_i=None):
     B = out_ids.numel()
     check(lib().me_sample_topk_topp(_ptr(logits), logits.stride(0), V, _ptr(special),

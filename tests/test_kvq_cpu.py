@@ -67,10 +67,11 @@ def test_refusals_of_the_cache():
                  lambda: c.attend(q, -2), lambda: c.attend(q, 3, rel=rel[:63]), lambda: c.attend(q, 3, rel=rel.half()), lambda: c.attend(q, 3, rel=rel.t()),
                  lambda: c.attend(q, 3, key_pad=pad[:, ::2]), lambda: c.attend(q, 3, key_pad=pad[:1]), lambda: c.attend(q, 3, key_pad=pad[:, :3].contiguous()),
                  lambda: c.attend(q, 3, out=q.half()), lambda: c.attend(q, 3, out=torch.zeros(1, 3, 32).expand(2, 3, 32)), lambda: c.attend(q, 3, nsplit=65),
-                 lambda: c.attend(q.transpose(0, 1), 3)):
+                 lambda: c.attend(q.transpose(0, 1), 3), lambda: c.append_attend(q, q, q.half(), 3), lambda: c.append_attend(q, q[:1], q[:1], 3),
+                 lambda: c.append_attend(q, q, q, -1), lambda: c.append_attend(q, q, q, 64), lambda: c.append_attend(q, q, torch.zeros(3, 2, 32).transpose(0, 1), 3)):
         with pytest.raises(RuntimeError, match="kv cache"):
             call()
-    for call in (lambda: c.write(k, k, 0), lambda: c.read(0, 5), lambda: c.attend(q, 3, rel=rel, key_pad=pad)):       # right, but no device
+    for call in (lambda: c.write(k, k, 0), lambda: c.read(0, 5), lambda: c.append_attend(q, q, q, 3), lambda: c.attend(q, 3, rel=rel, key_pad=pad)):       # right, but no device
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
 
@@ -102,6 +103,11 @@ def test_refusals_of_the_c_abi():
     assert need == 4 * 68 * 4
     assert attn(nsplit=4) == WS and attn(nsplit=4, part=P, part_bytes=need - 1) == WS and attn(out=None, part=P, part_bytes=68 * 4 - 4) == WS
     assert attn(B=0) == 0
+
+    def append(k=P, v=P, ldn=64, t=0, **kw):
+        return lib.me_kvq_append_attn(cache(**kw), P, 64, 64, k, v, ldn, 64, None, 0, None, 0, P, 64, 64, None, 0, 1, t, None, 0, _lib.ME_BF16, None)
+    assert append(k=None) == NULL and append(v=None) == NULL and append(t=-1) == SHAPE and append(t=32) == SHAPE and append(k=P + 2) == ALIGN and append(v=P + 4) == ALIGN
+    assert append(ldn=63) == ALIGN and append(B=0) == 0
     for rel in (0, 1):
         for b, h, n in ((1, 8, 1), (1, 8, 2048), (4, 8, 2048), (64, 16, 1999), (1, 1, 1 << 30), (10 ** 6, 8, 2048), (0, 1, 1)):
             assert 1 <= lib.me_kvq_splits(b, h, n, rel) <= 64

@@ -218,6 +218,51 @@ def test_attention_ragged_padded_and_empty_rows(T, dh, bits):
     assert torch.equal(out[1], full[1]) and torch.equal(out[5], full[5])
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dh", [32, 48, 64])
+@pytest.mark.parametrize("T", ["bf16", "f16", "f32"])
+def test_append_and_attend_in_one_launch(T, dh, bits):
+    """the cache afterwards is the one that write() leaves, bit for bit; the result is the formula over it"""
+    T, B, H, n = DT[T], 4, 5, 160
+    g = torch.Generator().manual_seed(dh + bits)
+    x = rows(B, n, H, dh, T, 17).cuda()
+    E = torch.randn(2048, dh, generator=g).to(T)
+    for pos in ([0, 1, 2, 31], [32, 63, 64, 127], [128, 129, 159, 100], 0, 133, [-1, 160, 400, 5]):
+        a, b = cache(B, H, n, dh, bits), cache(B, H, n, dh, bits)
+        for c in (a, b):
+            c.write(x[:, :, 1], x[:, :, 2], 0)
+        new = rows(B, 1, H, dh, T, 23).cuda()
+        kn, vn = new[:, 0, 1].contiguous(), new[:, 0, 2].contiguous()
+        p = pos if isinstance(pos, int) else torch.tensor(pos, dtype=torch.int32, device="cuda")
+        b.write(kn[:, None], vn[:, None], p)
+        q = torch.randn(B, H, dh, generator=g).to(T)
+        listed = [pos] * B if isinstance(pos, int) else [min(i, n - 1) for i in pos]
+        k, v = [t.cpu().double().transpose(1, 2) for t in b.read(0, n, torch.float32)]
+        for rel in (E, None):
+            pad = torch.rand(B, n, generator=g) < 0.2
+            pad[1, listed[1]] = True                              # the new key itself masked: written, not used
+            for ns, mask in ((0, None), (1, pad), (2, None), (7, pad)):
+                c = cache(B, H, n, dh, bits)
+                for m in ("k", "v", "k_scale", "v_scale"):
+                    getattr(c, m).copy_(getattr(a, m))
+                out = c.append_attend(q.cuda(), kn, vn, p, rel=None if rel is None else rel.cuda(), key_pad=None if mask is None else mask.cuda(), nsplit=ns)
+                for m in ("k", "v"):
+                    assert torch.equal(getattr(c, m), getattr(b, m)), (m, pos)
+                for m in ("k_scale", "v_scale"):
+                    assert torch.equal(getattr(c, m).view(torch.int16), getattr(b, m).view(torch.int16)), (m, pos)
+                check(out, q, k, v, listed, rel, mask, T, dh, bits)
+    # rows that are not numbers: held as such, and the result says so
+    kn[0, 0, 3], vn[1, 1, 0] = math.inf, math.nan
+    for ns in (1, 3):
+        c = cache(B, H, n, dh, bits)
+        c.write(x[:, :, 1], x[:, :, 2], 0)
+        out = c.append_attend(q.cuda(), kn, vn, 90, nsplit=ns).cpu()
+        assert bool(torch.isnan(out[0, 0]).all()) and bool(torch.isnan(out[1, 1]).all()) and bool(torch.isfinite(out[2:]).all())
+        d = cache(B, H, n, dh, bits)
+        out = d.append_attend(q.cuda(), kn, vn, 0, nsplit=ns).cpu()      # the only key
+        assert bool(torch.isnan(out[0, 0]).all()) and bool(torch.isfinite(out[2:]).all())
+
+
 def test_attention_values_that_are_not_numbers():
     c = cache(2, 2, 64, 64, 4)
     x = rows(2, 64, 2, 64, torch.bfloat16, 2)

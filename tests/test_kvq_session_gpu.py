@@ -105,7 +105,7 @@ def test_device_loops_are_the_single_steps(cd, bits, B):
         got = torch.cat([s2.greedy_run(first, n // 2, cond, special, use_graph=graph), ], 1)
         got = torch.cat([got, s2.greedy_run(got[:, -1], n - n // 2, cond, special, use_graph=graph)], 1)
         assert torch.equal(got, want), graph
-    assert s2.launches_per_token == (2 + 4 * (1 if B <= 8 else 2)) * 2 + 1 + (1 if B <= 8 else 2) + 1
+    assert s2.launches_per_token == (1 + 4 * (1 if B <= 8 else 2)) * 2 + 1 + (1 if B <= 8 else 2) + 1
     # sampled, with min-p
     ts = (torch.arange(cfg.vocab_size) % 7 == 0).cuda()
     uni = torch.rand(n, B, generator=torch.Generator().manual_seed(3)).cuda()
