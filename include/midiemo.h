@@ -170,6 +170,7 @@ enum {
     ME_WS_SUMSQ = 7,         /* me_sumsq ordered block sums: ME_SUMSQ_WS_BYTES, zero before the first use */
     ME_WS_RELU_MASK = 8,     /* me_gemm_nt_relu_mask sign mask: (M, N, K) = the product's; 0 = shape / dtype not served, use the gate */
     ME_WS_DEC_TOKEN = 9,     /* me_dec_token exchange records: (M, N, K) = (Mr, d_inner, d); zero before the first use */
+    ME_WS_SAMPLE = 11,       /* me_sample_minp(_step): (M, N, K) = (B, V, unused); 0 for V <= ME_SAMPLE_ONE_BLOCK */
     ME_WS_KVQ_ATTN = 10      /* me_kvq_attn partial records: (M, N, K) = (B * H, nsplit, dh) */
 };
 size_t me_workspace_bytes(int op, int M, int N, int K, int dtype);
@@ -520,7 +521,7 @@ int me_sample_step(const float* logits, int ld, int V, const int32_t* special, i
                    int top_k, float top_p, const float* u_table, int u_ld, const int32_t* pos, int pos0, int64_t* out_ids,
                    int32_t* n_choices, int B, void* stream);
 
-/* Sampling with min-p and for wide vocabularies (V <= ME_SAMPLE_MAX_VOCAB), one launch for the whole batch: the rules of
+/* Sampling with min-p and for wide vocabularies (V <= ME_SAMPLE_MAX_VOCAB), one launch for the whole batch (four beyond 8192 symbols): the rules of
  * me_sample_topk_topp with min-p behind them and the arithmetic in 64 bits.  NaN -> 0, ids in special[] -> -inf; entries in the order
  * (logit descending, index ascending); weight w = exp((x - max x) / temp[b]); kept are the entries that pass all of
  *   top_k  (> 0): the first top_k entries;
@@ -530,15 +531,17 @@ int me_sample_step(const float* logits, int ld, int V, const int32_t* special, i
  * out_ids[b] = the first kept entry at which the cumulative weight exceeds u[b] times the sum of the kept ones (u in [0, 1); a u of 1 and
  * more: the last one that has a weight); n_choices[b] (may be NULL) = number of kept entries.  A row with every logit -inf: id 0, 0 choices;
  * several +inf share the weight.  Cumulative weights are exact sums of weights rounded to 2^-45, so results do not depend on scheduling.
- * temp[b] must be positive and finite.
+ * temp[b] must be positive and finite.  ws: me_workspace_bytes(ME_WS_SAMPLE, B, V, 0, 0) bytes, 16-byte aligned, uninitialised, private to the call
+ * until it has run (NULL where that is 0).
  * me_sample_minp_step is the same for a step of a device-resident loop (arguments of me_sample_step). */
 #define ME_SAMPLE_MAX_VOCAB (1 << 18)
+#define ME_SAMPLE_ONE_BLOCK 8192       /* widest row that needs no workspace */
 int me_sample_minp(const float* logits, int ld, int V, const int32_t* special, int n_special, const float* temp, int top_k, float top_p,
-                   float min_p, const float* u, int64_t* out_ids, int32_t* n_choices, int B, void* stream);
+                   float min_p, const float* u, int64_t* out_ids, int32_t* n_choices, int B, void* ws, size_t ws_bytes, void* stream);
 int me_sample_minp_step(const float* logits, int ld, int V, const int32_t* special, int n_special, const int64_t* prev_tok,
                         const uint8_t* is_timeshift, float* repeat_counts, float temp_note, float temp_rest, float penalty_coeff, int top_k,
                         float top_p, float min_p, const float* u_table, int u_ld, const int32_t* pos, int pos0, int64_t* out_ids,
-                        int32_t* n_choices, int B, void* stream);
+                        int32_t* n_choices, int B, void* ws, size_t ws_bytes, void* stream);
 
 /* Device-side decode bookkeeping: history[b][*pos] = tok[b] (int64 [B][ld_hist]); *pos += 1.
  * With me_embed_fwd(pos_dev) and the t_dev arguments of me_dec_* a greedy decode step has no host-side state

@@ -248,6 +248,7 @@ ME_DEV bool me_keep(uint64_t seed, uint32_t site, uint64_t idx, uint32_t thr16) 
 // word) followed by the 8-byte exchange records of ME_DEC_TOKEN_ROWS sequences: s2, s1, att [rows][d]; qkv [rows][3d]; hid [rows][d_inner];
 // attention partials [rows * H][nsplit <= 8][dh + 2] <= rows * 8 * (d + d / 16 + 2) (dh >= 32)
 #define ME_DEC_TOKEN_ROWS 4
+size_t me_sample_ws_bytes(int B, int V);    // me_sample.hip
 static inline size_t me_dec_token_ws_bytes(int d, int d_inner) {
     return 256 + 8 * ((size_t)ME_DEC_TOKEN_ROWS * d * 6 + (size_t)ME_DEC_TOKEN_ROWS * d_inner + (size_t)ME_DEC_TOKEN_ROWS * 8 * (d + d / 16 + 2));
 }

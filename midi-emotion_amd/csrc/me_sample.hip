@@ -4,21 +4,30 @@
 // of the four rules keeps a prefix of that order, so the kept set is the shortest of them and what is needed are ranks and
 // cumulative weights at a few places of the order, not the order itself: nothing is sorted.  Two searches are enough,
 //     mass of the first r entries (top-k)      and      first entry whose cumulative weight exceeds T (nucleus, draw),
-// and both walk one histogram of 2048 bins over (max x - x) / temperature and then look into the single bin that holds the border.
+// and both walk one histogram of 1024 bins over (max x - x) / temperature and then look into the single bin that holds the border.
 //
 // Weights are whole multiples of 2^-45 in 64 bits (computed in f64): their sums do not depend on the order in which LDS
 // atomics arrive, so a call repeats bit for bit, and 2^18 of them cannot overflow.  A pick next to a border between two entries
 // needs about that many bits: the cumulative weights of a flat row lie 2^-18 apart, and f32 sums would move one pick in a few thousand.
+//
+// What bounds it: the f64 weight of every entry, about 30 instructions, on however many CUs share a row.  Rows of up to 8192 symbols take
+// one block (the row stays in LDS).  Wider ones take four launches: the chunks' maxima; the chunks' histograms; the members of the
+// bins that can hold one of the borders (known up to a bin or two from the histogram alone), gathered by all chunks; and one block per row
+// that finishes on those few entries.
 #include "me_common.h"
+#include <algorithm>
 #include <math.h>
 
 namespace {
 
 typedef unsigned long long u64;
 
-constexpr int NB = 2048;                    // bins of a search level
-constexpr int NL = 1024;                    // entries of a bin that are compared with each other directly
+constexpr int NB = 1024;                    // bins of a search level; level 0: 32 per unit of (max - x) / temperature
+constexpr int NL = 512;                     // entries of a bin that are compared with each other directly
+constexpr int GL = 4096;                    // gathered entries of a wide row
 constexpr int FRAC = 45;                    // weight unit 2^-45
+constexpr int ONE_BLOCK = ME_SAMPLE_ONE_BLOCK;
+constexpr int MAX_SPLIT = 16;               // chunks of a wide row at most: every later block reads all chunks' histograms
 
 struct SampleArgs {
     const float* logits; int ld, V;
@@ -31,7 +40,35 @@ struct SampleArgs {
     // a step of a device-resident loop (prev != NULL): temperature from the token just fed, uniform from a table, repeat counter
     const int64_t* prev; const uint8_t* is_timeshift; float* repeats; const int32_t* pos;
     int pos0, u_ld; float temp_note, temp_rest, penalty;
+    // wide rows: the workspace, the chunks
+    char* ws; int splits, chunk, B;
 };
+
+// workspace of a wide row (16-byte multiples); written before it is read by every call
+struct RowWs {
+    u64* mass;                              // [splits][NB]
+    uint32_t* cnt;                          // [splits][NB]
+    u64* m_keep;                            // [MAX_SPLIT]
+    uint32_t* n_keep;                       // [MAX_SPLIT]
+    float* mx;                              // [MAX_SPLIT]
+    uint32_t* n_list;                       // [4]
+    int* ranges;                            // [8]: the gathered bins
+    u64* list;                              // [GL]
+};
+__host__ __device__ inline size_t row_ws_bytes(int splits) { return (size_t)splits * NB * 12 + MAX_SPLIT * 16 + 16 + 32 + GL * 8; }
+ME_DEV RowWs row_ws(const SampleArgs& a, int b) {
+    char* p = a.ws + (size_t)b * row_ws_bytes(a.splits);
+    RowWs w;
+    w.mass = reinterpret_cast<u64*>(p); p += (size_t)a.splits * NB * 8;
+    w.cnt = reinterpret_cast<uint32_t*>(p); p += (size_t)a.splits * NB * 4;
+    w.m_keep = reinterpret_cast<u64*>(p); p += MAX_SPLIT * 8;
+    w.n_keep = reinterpret_cast<uint32_t*>(p); p += MAX_SPLIT * 4;
+    w.mx = reinterpret_cast<float*>(p); p += MAX_SPLIT * 4;
+    w.n_list = reinterpret_cast<uint32_t*>(p); p += 16;
+    w.ranges = reinterpret_cast<int*>(p); p += 32;
+    w.list = reinterpret_cast<u64*>(p);
+    return w;
+}
 
 // order-preserving image of (x, j): greater = earlier in the order
 ME_DEV u64 word_of(float x, int j) {
@@ -39,21 +76,62 @@ ME_DEV u64 word_of(float x, int j) {
     b ^= (b >> 31) ? 0xffffffffu : 0x80000000u;
     return ((u64)b << 32) | (0xffffffffu - (uint32_t)j);
 }
+ME_DEV float value_of(u64 word) {
+    uint32_t b = (uint32_t)(word >> 32);
+    b ^= (b >> 31) ? 0x80000000u : 0xffffffffu;
+    return __uint_as_float(b);
+}
+ME_DEV int index_of(u64 word) { return (int)(0xffffffffu - (uint32_t)word); }
 
-// 2^y (y <= 0) in units of 2^-45, rounded to nearest: 2^f on [-1/2, 1/2] by its Taylor series (13 terms: below 2^-50), the
-// scaling exact, and the conversion by adding 2^52 (the integer is then the mantissa)
-ME_DEV u64 weight_of(double y) {
-    if (!(y > -(double)(FRAC + 2))) return 0;
-    const double n = rint(y), r = (y - n) * 0.693147180559945309417;
-    double p = 1.0 / 479001600.0;
-    p = fma(p, r, 1.0 / 39916800.0); p = fma(p, r, 1.0 / 3628800.0); p = fma(p, r, 1.0 / 362880.0); p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);     p = fma(p, r, 1.0 / 720.0);     p = fma(p, r, 1.0 / 120.0);    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);        p = fma(p, r, 0.5);             p = fma(p, r, 1.0);            p = fma(p, r, 1.0);
-    const double scale = __longlong_as_double((long long)((int)n + FRAC + 1023) << 52);
-    return (u64)(__double_as_longlong(fma(p, scale, 0x1p52)) - __double_as_longlong(0x1p52));
+// a row's scale: exponents y = (x - max) / temperature * log2 e, weights 2^y, bins
+struct Scale {
+    float mx, bin_c;
+    double c;                               // 32 log2 e / temperature
+    const double* tab;                      // 2^(i / 32)
+    ME_DEV void set(float m, float temp, const double* t) {
+        mx = m;
+        bin_c = (float)NB / 32.f / temp;
+        c = 32 * 1.4426950408889634074 / (double)temp;
+        tab = t;
+    }
+    // 32 y; equal values (two infinities too) give 0
+    ME_DEV double exponent(float v) const { return v == mx ? 0.0 : ((double)v - (double)mx) * c; }
+    ME_DEV int bin(float v) const { return v == mx ? 0 : (int)fminf((mx - v) * bin_c, (float)(NB - 1)); }
+    // 2^(e / 32) (e <= 0) in units of 2^-45, rounded to nearest: table times the Taylor series of 2^f, |f| <= 1/64 (6 terms: below
+    // 2^-48), scaled exactly, converted by adding 2^52 (the integer is then the mantissa)
+    ME_DEV u64 weight(double e) const {
+        if (!(e > -32.0 * (FRAC + 2))) return 0;
+        const double k = rint(e), r = (e - k) * (0.693147180559945309417 / 32);
+        const int n = (int)k;
+        double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+        p = fma(p, r, 1.0 / 6.0); p = fma(p, r, 0.5); p = fma(p, r, 1.0); p = fma(p, r, 1.0);
+        const double scale = __longlong_as_double((long long)((n >> 5) + FRAC + 1023) << 52);
+        return (u64)(__double_as_longlong(fma(p * tab[n & 31], scale, 0x1p52)) - __double_as_longlong(0x1p52));
+    }
+    // what min-p and a positive weight leave: exp() of 64 bits is 0 from 2^-1075 on
+    ME_DEV static bool keeps(double e, double y_min) { return e >= 32 * y_min && e > -1075.0 * 32; }
+};
+
+// temperature and uniform of a row (step form: the f32 operations of generate.py's sampling_temperature(), unfused)
+ME_DEV float row_temp(const SampleArgs& a, int b) {
+    if (!a.prev) return a.temp[b];
+    const int64_t pt = a.prev[b];
+    float temp = pt >= 0 && pt < a.V && a.is_timeshift[pt] ? a.temp_note : a.temp_rest;
+    if (a.penalty > 0.f) {
+        const float mult = fmaxf(__fmul_rn(logf(__fdiv_rn(__fadd_rn(a.repeats[b], 1.f), 4.f)), a.penalty), 0.f);
+        temp = __fadd_rn(temp, __fmul_rn(mult, temp));
+    }
+    return temp;
+}
+ME_DEV float row_u(const SampleArgs& a, int b) { return a.prev ? a.u[(size_t)(a.pos[0] - a.pos0) * a.u_ld + b] : a.u[b]; }
+ME_DEV void finish(const SampleArgs& a, int b, int64_t id, int n) {       // one thread
+    a.out[b] = id;
+    if (a.choices) a.choices[b] = n;
+    if (a.prev) { const float rc = a.repeats[b]; a.repeats[b] = n <= 2 ? rc + 1.f : floorf(rc * 0.5f); }      // generate.py:186-189
 }
 
 template <int NT> struct Shared {
+    double tab[32];
     uint32_t cnt[NB];                       // level 0: per bin, then entries before it
     u64 mass[NB];
     uint32_t cnt1[NB];                      // deeper levels
@@ -86,6 +164,14 @@ template <int NT> ME_DEV u64 block_max64(Shared<NT>& s, u64 v) {
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) t = s.r64[w] > t ? s.r64[w] : t;
     return t;
+}
+template <int NT> ME_DEV float block_max(Shared<NT>& s, float v) {
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) s.r32[threadIdx.x >> 6] = __float_as_uint(v);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) v = fmaxf(v, __uint_as_float(s.r32[w]));
+    return v;
 }
 
 // per-bin counts and masses -> what lies before each bin; returns the totals
@@ -126,196 +212,136 @@ template <int NT> ME_DEV void scan_bins(Shared<NT>& s, uint32_t* cnt, u64* mass,
     __syncthreads();
 }
 
-// NT threads per row.  ROW: the row stays in LDS after the first pass (V <= ROW_MAX); else every pass reads it again (from L2)
-constexpr int ROW_MAX = 26624;
-template <int NT, bool ROW>
-__global__ __launch_bounds__(NT) void sample_minp_kernel(const SampleArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    Shared<NT>& s = *reinterpret_cast<Shared<NT>*>(smem);
-    uint32_t* barred = reinterpret_cast<uint32_t*>(smem + sizeof(Shared<NT>));        // !ROW: one bit per symbol
-    float* row = reinterpret_cast<float*>(smem + sizeof(Shared<NT>));                 // ROW: the logits
-    const int tid = threadIdx.x, b = blockIdx.x, V = a.V;
-    const float* lg = a.logits + (size_t)b * a.ld;
-    constexpr int U = ROW ? 4 : 8;                            // entries of a thread in flight
-
-    // every entry once: NaN -> 0, special ids -> -inf
-    auto each = [&](auto&& f) {
-        for (int j0 = tid; j0 < V; j0 += NT * U) {
-            float x[U];
-#pragma unroll
-            for (int q = 0; q < U; ++q) { const int j = min(j0 + q * NT, V - 1); x[q] = ROW ? row[j] : lg[j]; }
-#pragma unroll
-            for (int q = 0; q < U; ++q) {
-                const int j = j0 + q * NT;
-                if (j < V) {
-                    float v = x[q];
-                    if (!ROW) { if (v != v) v = 0.f; if ((barred[j >> 5] >> (j & 31)) & 1u) v = -INFINITY; }
-                    f(v, j);
-                }
-                __builtin_amdgcn_sched_barrier(0);            // the entries' f64 chains stay apart (the waves hide them): few registers
-            }
-        }
-    };
-    if constexpr (ROW) {
-        constexpr int L = 8;
-        for (int j0 = tid; j0 < V; j0 += NT * L) {
-            float x[L];
-#pragma unroll
-            for (int q = 0; q < L; ++q) x[q] = lg[min(j0 + q * NT, V - 1)];
-#pragma unroll
-            for (int q = 0; q < L; ++q) if (j0 + q * NT < V) row[j0 + q * NT] = x[q] != x[q] ? 0.f : x[q];
-        }
-        __syncthreads();
-        for (int i = tid; i < a.n_special; i += NT) { const int j = a.special[i]; if (j >= 0 && j < V) row[j] = -INFINITY; }
-    } else {
-        for (int i = tid; i < (V + 31) / 32; i += NT) barred[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < a.n_special; i += NT) { const int j = a.special[i]; if (j >= 0 && j < V) atomicOr(&barred[j >> 5], 1u << (j & 31)); }
+// the sums of all chunks' histograms, scanned; what min-p keeps
+template <int NT> ME_DEV void load_hist(Shared<NT>& s, const SampleArgs& a, const RowWs& w, uint32_t& n_all, u64& m_all, uint32_t& n_keep, u64& m_keep) {
+    for (int i = threadIdx.x; i < NB; i += NT) {
+        uint32_t c = 0;
+        u64 m = 0;
+#pragma unroll 4
+        for (int q = 0; q < a.splits; ++q) { c += w.cnt[q * NB + i]; m += w.mass[q * NB + i]; }
+        s.cnt[i] = c;
+        s.mass[i] = m;
     }
+    n_keep = 0; m_keep = 0;
+    for (int q = 0; q < a.splits; ++q) { n_keep += w.n_keep[q]; m_keep += w.m_keep[q]; }
     __syncthreads();
-
-    // ---- temperature and uniform of the row (step form: the f32 operations of generate.py's sampling_temperature(), unfused)
-    float temp, u;
-    if (a.prev) {
-        const int64_t pt = a.prev[b];
-        temp = pt >= 0 && pt < V && a.is_timeshift[pt] ? a.temp_note : a.temp_rest;
-        if (a.penalty > 0.f) {
-            const float mult = fmaxf(__fmul_rn(logf(__fdiv_rn(__fadd_rn(a.repeats[b], 1.f), 4.f)), a.penalty), 0.f);
-            temp = __fadd_rn(temp, __fmul_rn(mult, temp));
-        }
-        u = a.u[(size_t)(a.pos[0] - a.pos0) * a.u_ld + b];
-    } else {
-        temp = a.temp[b];
-        u = a.u[b];
-    }
-
-    float mx = -INFINITY;
-    each([&](float v, int) { mx = fmaxf(mx, v); });
-    mx = wave_max(mx);
-    if ((tid & 63) == 0) s.r32[tid >> 6] = __float_as_uint(mx);
-    for (int i = tid; i < NB; i += NT) { s.cnt[i] = 0; s.mass[i] = 0; }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) mx = fmaxf(mx, __uint_as_float(s.r32[w]));
-
-    auto finish = [&](int64_t id, int n) {                    // one thread
-        a.out[b] = id;
-        if (a.choices) a.choices[b] = n;
-        if (a.prev) { const float rc = a.repeats[b]; a.repeats[b] = n <= 2 ? rc + 1.f : floorf(rc * 0.5f); }      // generate.py:186-189
-    };
-    if (mx == -INFINITY) {                                    // nothing to choose from
-        if (tid == 0) finish(0, 0);
-        return;
-    }
-    // exponents: y = (x - max) / temperature * log2 e in f64; equal values (two infinities too) give 0
-    const double c2 = 1.4426950408889634074 / (double)temp;
-    const float bin_c = (float)NB / 32.f / temp;
-    auto exponent = [&](float v) -> double { return v == mx ? 0.0 : ((double)v - (double)mx) * c2; };
-    auto bin_of = [&](float v) -> int { return v == mx ? 0 : (int)fminf((mx - v) * bin_c, (float)(NB - 1)); };
-
-    // ---- histogram; what min-p and a positive weight leave is a threshold on y: counted on the way
-    const double y_min = a.y_min;
-    uint32_t n_keep = 0;
-    u64 m_keep = 0;
-    each([&](float v, int) {
-        const double y = exponent(v);
-        const u64 w = weight_of(y);
-        const bool keep = y >= y_min && y > -1075.0;          // exp() of 64 bits is 0 from 2^-1075 on
-        n_keep += keep;
-        m_keep += keep ? w : 0;
-        const int bin = bin_of(v);
-        atomicAdd(&s.cnt[bin], 1u);
-        if (w) atomicAdd(&s.mass[bin], w);
-    });
-    n_keep = (uint32_t)block_sum64(s, (u64)n_keep);
-    m_keep = block_sum64(s, m_keep);
-    uint32_t n_all;
-    u64 m_all;
     scan_bins<NT>(s, s.cnt, s.mass, n_all, m_all);
+}
 
-    // ---- search: by_rank: the mass of the first `rank` entries; else the first entry whose cumulative weight exceeds `limit`
-    //      (its word, its rank, the mass before it)
-    auto search = [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& before) {
-        uint32_t* cnt = s.cnt;
-        u64* mass = s.mass;
-        uint32_t total = n_all, c0 = 0;                       // entries and mass before the window of this level
-        u64 mtotal = m_all, m0 = 0;
-        u64 hi = 0, lo = 0;
-        int shift = 0, level = 0, bin0 = 0;
-        while (true) {
-            for (int i = tid; i < NB; i += NT) {
-                const uint32_t cb = c0 + cnt[i], ce = c0 + (i + 1 < NB ? cnt[i + 1] : total);
-                const u64 mb = m0 + mass[i], me = m0 + (i + 1 < NB ? mass[i + 1] : mtotal);
-                if (by_rank ? (cb < rank && rank <= ce) : (mb <= limit && limit < me)) s.found_bin = (uint32_t)i;
+// entries [j0, j1) of a row, once each: NaN -> 0, barred ids (bit j - j0) -> -inf; f(value, index)
+template <int NT, int U, typename F> ME_DEV void each_entry(const float* lg, int j0, int j1, const uint32_t* barred, F&& f) {
+    for (int i0 = j0 + (int)threadIdx.x; i0 < j1; i0 += NT * U) {
+        float x[U];
+#pragma unroll
+        for (int q = 0; q < U; ++q) x[q] = lg[min(i0 + q * NT, j1 - 1)];
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            const int j = i0 + q * NT;
+            if (j < j1) {
+                float v = x[q];
+                if (v != v) v = 0.f;
+                if (barred && ((barred[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u)) v = -INFINITY;
+                f(v, j);
             }
-            __syncthreads();
-            const int bin = (int)s.found_bin;
-            const uint32_t cb = c0 + cnt[bin], n = c0 + (bin + 1 < NB ? cnt[bin + 1] : total) - cb;
-            const u64 mb = m0 + mass[bin];
-            if (level == 0) bin0 = bin;
-            else { const u64 top = hi - ((u64)bin << shift); lo = max(lo, top - (((u64)1 << shift) - 1)); hi = top; }
-            c0 = cb;
-            m0 = mb;
-            __syncthreads();                                  // found_bin, cnt, mass have been read
-            auto inside = [&](float v, u64 w) { return level == 0 ? bin_of(v) == bin0 : w <= hi && w >= lo; };
-            if (n <= NL) {
-                if (tid == 0) s.n_list = 0;
-                __syncthreads();
-                each([&](float v, int j) {
-                    const u64 w = word_of(v, j);
-                    if (inside(v, w)) s.lw[atomicAdd(&s.n_list, 1u)] = w;
-                });
-                __syncthreads();
-                for (uint32_t e = tid; e < n; e += NT) {
-                    uint32_t bits = (uint32_t)(s.lw[e] >> 32);
-                    bits ^= (bits >> 31) ? 0x80000000u : 0xffffffffu;
-                    s.lm[e] = weight_of(exponent(__uint_as_float(bits)));
-                }
-                __syncthreads();
-                for (uint32_t e = tid; e < n; e += NT) {
-                    const u64 me = s.lw[e], own = s.lm[e];
-                    uint32_t r = 0;
-                    u64 cum = own;
-#pragma clang loop unroll_count(4)
-                    for (uint32_t k = 0; k < n; ++k) { const bool ahead = s.lw[k] > me; r += ahead; cum += ahead ? s.lm[k] : 0; }
-                    const bool hit = by_rank ? c0 + r + 1 == rank : (m0 + cum > limit && m0 + cum - own <= limit);
-                    if (hit) { s.found_word = me; s.found_rank = c0 + r; s.found_mass = by_rank ? m0 + cum : m0 + cum - own; }
-                }
-                __syncthreads();
-                word = s.found_word;
-                at = s.found_rank;
-                before = s.found_mass;
-                __syncthreads();
-                return;
-            }
-            // too many for that: the entries between the bin's first and last word, cut into 2048 pieces of the word's range (words
-            // differ, so a few levels end at one entry each)
-            u64 wmax = 0, wmin = 0;                           // wmin as the maximum of the complement
-            each([&](float v, int j) { const u64 w = word_of(v, j); if (inside(v, w)) { wmax = max(wmax, w); wmin = max(wmin, ~w); } });
-            hi = block_max64(s, wmax);
-            lo = ~block_max64(s, wmin);
-            level = 1;
-            shift = 0;
-            while (((hi - lo) >> shift) >= NB) ++shift;
-            for (int i = tid; i < NB; i += NT) { s.cnt1[i] = 0; s.mass1[i] = 0; }
+            __builtin_amdgcn_sched_barrier(0);                // the entries' f64 chains stay apart (the waves hide them): few registers
+        }
+    }
+}
+template <int NT> ME_DEV const uint32_t* bar_ids(const SampleArgs& a, uint32_t* bits, int j0, int j1) {
+    if (a.n_special <= 0) return nullptr;                     // uniform
+    for (int i = threadIdx.x; i < (j1 - j0 + 31) / 32; i += NT) bits[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.n_special; i += NT) { const int j = a.special[i]; if (j >= j0 && j < j1) atomicOr(&bits[(j - j0) >> 5], 1u << ((j - j0) & 31)); }
+    __syncthreads();
+    return bits;
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// the search over a scanned histogram and the entries that `each` walks.  by_rank: the mass of the first `rank` entries; else the
+// first entry whose cumulative weight exceeds `limit` (its word, its rank, the mass before it).
+// ---------------------------------------------------------------------------------------------------------
+template <int NT, typename EACH>
+ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, uint32_t n_all, u64 m_all, bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& before) {
+    const int tid = threadIdx.x;
+    uint32_t* cnt = s.cnt;
+    u64* mass = s.mass;
+    uint32_t total = n_all, c0 = 0;                           // entries and mass before the window of this level
+    u64 mtotal = m_all, m0 = 0;
+    u64 hi = 0, lo = 0;
+    int shift = 0, level = 0, bin0 = 0;
+#pragma clang loop unroll(disable)
+    while (true) {
+        for (int i = tid; i < NB; i += NT) {
+            const uint32_t cb = c0 + cnt[i], ce = c0 + (i + 1 < NB ? cnt[i + 1] : total);
+            const u64 mb = m0 + mass[i], me = m0 + (i + 1 < NB ? mass[i + 1] : mtotal);
+            if (by_rank ? (cb < rank && rank <= ce) : (mb <= limit && limit < me)) s.found_bin = (uint32_t)i;
+        }
+        __syncthreads();
+        const int bin = (int)s.found_bin;
+        const uint32_t cb = c0 + cnt[bin], n = c0 + (bin + 1 < NB ? cnt[bin + 1] : total) - cb;
+        const u64 mb = m0 + mass[bin];
+        if (level == 0) bin0 = bin;
+        else { const u64 top = hi - ((u64)bin << shift); lo = max(lo, top - (((u64)1 << shift) - 1)); hi = top; }
+        c0 = cb;
+        m0 = mb;
+        __syncthreads();                                      // found_bin, cnt, mass have been read
+        auto inside = [&](float v, u64 w) { return level == 0 ? sc.bin(v) == bin0 : w <= hi && w >= lo; };
+        if (n <= NL) {
+            if (tid == 0) s.n_list = 0;
             __syncthreads();
             each([&](float v, int j) {
                 const u64 w = word_of(v, j);
-                if (w <= hi && w >= lo) {
-                    const int i = (int)((hi - w) >> shift);
-                    const u64 m = weight_of(exponent(v));
-                    atomicAdd(&s.cnt1[i], 1u);
-                    if (m) atomicAdd(&s.mass1[i], m);
-                }
+                if (inside(v, w)) s.lw[atomicAdd(&s.n_list, 1u)] = w;
             });
             __syncthreads();
-            cnt = s.cnt1;
-            mass = s.mass1;
-            scan_bins<NT>(s, cnt, mass, total, mtotal);
+            for (uint32_t e = tid; e < n; e += NT) s.lm[e] = sc.weight(sc.exponent(value_of(s.lw[e])));
+            __syncthreads();
+            for (uint32_t e = tid; e < n; e += NT) {
+                const u64 me = s.lw[e], own = s.lm[e];
+                uint32_t r = 0;
+                u64 cum = own;
+#pragma clang loop unroll_count(4)
+                for (uint32_t k = 0; k < n; ++k) { const bool ahead = s.lw[k] > me; r += ahead; cum += ahead ? s.lm[k] : 0; }
+                const bool hit = by_rank ? c0 + r + 1 == rank : (m0 + cum > limit && m0 + cum - own <= limit);
+                if (hit) { s.found_word = me; s.found_rank = c0 + r; s.found_mass = by_rank ? m0 + cum : m0 + cum - own; }
+            }
+            __syncthreads();
+            word = s.found_word;
+            at = s.found_rank;
+            before = s.found_mass;
+            __syncthreads();
+            return;
         }
-    };
+        // too many for that: the entries between the bin's first and last word, cut into 1024 pieces of the word's range (words
+        // differ, so a few levels end at one entry each)
+        u64 wmax = 0, wmin = 0;                               // wmin as the maximum of the complement
+        each([&](float v, int j) { const u64 w = word_of(v, j); if (inside(v, w)) { wmax = max(wmax, w); wmin = max(wmin, ~w); } });
+        hi = block_max64(s, wmax);
+        lo = ~block_max64(s, wmin);
+        level = 1;
+        shift = 0;
+        while (((hi - lo) >> shift) >= NB) ++shift;
+        for (int i = tid; i < NB; i += NT) { s.cnt1[i] = 0; s.mass1[i] = 0; }
+        __syncthreads();
+        each([&](float v, int j) {
+            const u64 w = word_of(v, j);
+            if (w <= hi && w >= lo) {
+                const int i = (int)((hi - w) >> shift);
+                const u64 m = sc.weight(sc.exponent(v));
+                atomicAdd(&s.cnt1[i], 1u);
+                if (m) atomicAdd(&s.mass1[i], m);
+            }
+        });
+        __syncthreads();
+        cnt = s.cnt1;
+        mass = s.mass1;
+        scan_bins<NT>(s, cnt, mass, total, mtotal);
+    }
+}
 
-    // ---- top-k, then min-p, then the nucleus, then the draw
+// ---- top-k, then min-p, then the nucleus, then the draw.  searcher(by_rank, rank, limit, word, at, mass)
+template <typename S>
+ME_DEV void choose(const SampleArgs& a, int b, float u, uint32_t n_all, u64 m_all, uint32_t n_keep, u64 m_keep, S&& searcher) {
     u64 word = 0, mass = 0, tot = m_all, tot_k = m_all, limit = 0;
     uint32_t at = 0, n = n_all;
 #pragma clang loop unroll(disable)
@@ -332,58 +358,326 @@ __global__ __launch_bounds__(NT) void sample_minp_kernel(const SampleArgs a) {
             const double ut = u > 0.f ? (double)u * (double)tot : 0.0;
             limit = ut < (double)tot ? min((u64)ut, tot - 1) : tot - 1;           // u >= 1: the last entry that has a weight
         }
-        search(phase == 0, n, limit, word, at, mass);
+        searcher(phase == 0, n, limit, word, at, mass);
         if (phase == 0) tot = mass;
         if (phase == 1) { n = at > 0 ? at : 1; tot = at > 0 ? mass : (u64)1 << FRAC; }        // its first entry always stays
     }
-    if (tid == 0) finish((int64_t)(0xffffffffu - (uint32_t)word), (int)n);
+    if (threadIdx.x == 0) finish(a, b, index_of(word), (int)n);
 }
 
-template <int NT, bool ROW> int launch(const SampleArgs& a, int B, hipStream_t st) {
-    const size_t lds = sizeof(Shared<NT>) + (ROW ? (size_t)a.V * 4 : (size_t)(a.V + 31) / 32 * 4);
-    static bool raised[64] = {};                              // per device: more than 64 KB of LDS has been allowed
+// ---------------------------------------------------------------------------------------------------------
+// rows of up to ONE_BLOCK symbols: one block, the row in LDS
+// ---------------------------------------------------------------------------------------------------------
+template <int NT>
+__global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    Shared<NT>& s = *reinterpret_cast<Shared<NT>*>(smem);
+    float* row = reinterpret_cast<float*>(smem + sizeof(Shared<NT>));
+    const int tid = threadIdx.x, b = blockIdx.x, V = a.V;
+    const float* lg = a.logits + (size_t)b * a.ld;
+    const float temp = row_temp(a, b), u = row_u(a, b);
+    constexpr int L = 8;
+    for (int j0 = tid; j0 < V; j0 += NT * L) {
+        float x[L];
+#pragma unroll
+        for (int q = 0; q < L; ++q) x[q] = lg[min(j0 + q * NT, V - 1)];
+#pragma unroll
+        for (int q = 0; q < L; ++q) if (j0 + q * NT < V) row[j0 + q * NT] = x[q] != x[q] ? 0.f : x[q];
+    }
+    if (tid < 32) s.tab[tid] = exp2(tid * (1.0 / 32));
+    for (int i = tid; i < NB; i += NT) { s.cnt[i] = 0; s.mass[i] = 0; }
+    __syncthreads();
+    for (int i = tid; i < a.n_special; i += NT) { const int j = a.special[i]; if (j >= 0 && j < V) row[j] = -INFINITY; }
+    __syncthreads();
+    float mx = -INFINITY;
+    for (int j = tid; j < V; j += NT) mx = fmaxf(mx, row[j]);
+    mx = block_max<NT>(s, mx);
+    if (mx == -INFINITY) {                                    // nothing to choose from
+        if (tid == 0) finish(a, b, 0, 0);
+        return;
+    }
+    Scale sc;
+    sc.set(mx, temp, s.tab);
+    auto each = [&](auto&& f) { each_entry<NT, 4>(row, 0, V, nullptr, f); };
+    uint32_t n_keep = 0, n_all;
+    u64 m_keep = 0, m_all;
+    each([&](float v, int) {
+        const double e = sc.exponent(v);
+        const u64 w = sc.weight(e);
+        const bool keep = Scale::keeps(e, a.y_min);
+        n_keep += keep;
+        m_keep += keep ? w : 0;
+        const int bin = sc.bin(v);
+        atomicAdd(&s.cnt[bin], 1u);
+        if (w) atomicAdd(&s.mass[bin], w);
+    });
+    n_keep = (uint32_t)block_sum64(s, (u64)n_keep);
+    m_keep = block_sum64(s, m_keep);
+    scan_bins<NT>(s, s.cnt, s.mass, n_all, m_all);
+    choose(a, b, u, n_all, m_all, n_keep, m_keep, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
+        search<NT>(s, sc, each, n_all, m_all, by_rank, rank, limit, word, at, mass);
+    });
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// wider rows: grid (splits, B) blocks of a chunk each
+// ---------------------------------------------------------------------------------------------------------
+constexpr int WT = 512;                                       // threads of a chunk's block
+
+__global__ __launch_bounds__(WT) void sample_max_kernel(const SampleArgs a) {
+    extern __shared__ uint32_t bits[];
+    __shared__ float red[WT / 64];
+    const int b = blockIdx.y, j0 = blockIdx.x * a.chunk, j1 = min(j0 + a.chunk, a.V);
+    const RowWs w = row_ws(a, b);
+    const uint32_t* barred = bar_ids<WT>(a, bits, j0, j1);
+    float mx = -INFINITY;
+    each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int) { mx = fmaxf(mx, v); });
+    mx = wave_max(mx);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < WT / 64; ++i) mx = fmaxf(mx, red[i]);
+        w.mx[blockIdx.x] = mx;
+        if (blockIdx.x == 0) w.n_list[0] = 0;
+    }
+}
+ME_DEV float row_max(const SampleArgs& a, const RowWs& w) {
+    float mx = -INFINITY;
+    for (int q = 0; q < a.splits; ++q) mx = fmaxf(mx, w.mx[q]);
+    return mx;
+}
+
+__global__ __launch_bounds__(WT) void sample_hist_kernel(const SampleArgs a) {
+    extern __shared__ uint32_t bits[];
+    __shared__ Shared<WT> s;
+    const int tid = threadIdx.x, b = blockIdx.y, j0 = blockIdx.x * a.chunk, j1 = min(j0 + a.chunk, a.V);
+    const RowWs w = row_ws(a, b);
+    if (tid < 32) s.tab[tid] = exp2(tid * (1.0 / 32));
+    for (int i = tid; i < NB; i += WT) { s.cnt[i] = 0; s.mass[i] = 0; }
+    const uint32_t* barred = bar_ids<WT>(a, bits, j0, j1);
+    const float mx = row_max(a, w);
+    if (mx == -INFINITY) return;                              // the last launch sees it too
+    Scale sc;
+    sc.set(mx, row_temp(a, b), s.tab);
+    __syncthreads();
+    uint32_t n_keep = 0;
+    u64 m_keep = 0;
+    each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int) {
+        const double e = sc.exponent(v);
+        const u64 m = sc.weight(e);
+        const bool keep = Scale::keeps(e, a.y_min);
+        n_keep += keep;
+        m_keep += keep ? m : 0;
+        const int bin = sc.bin(v);
+        atomicAdd(&s.cnt[bin], 1u);
+        if (m) atomicAdd(&s.mass[bin], m);
+    });
+    n_keep = (uint32_t)block_sum64(s, (u64)n_keep);
+    m_keep = block_sum64(s, m_keep);
+    if (tid == 0) { w.n_keep[blockIdx.x] = n_keep; w.m_keep[blockIdx.x] = m_keep; }
+    for (int i = tid; i < NB; i += WT) { w.cnt[blockIdx.x * NB + i] = s.cnt[i]; w.mass[blockIdx.x * NB + i] = s.mass[i]; }
+}
+
+// the bins that can hold a border, from the histogram alone: each search ends in a known bin, and the mass inside the
+// bins of the earlier searches bounds the limits of the later ones.  Up to three ranges of bins.
+template <int NT> ME_DEV void border_bins(Shared<NT>& s, const SampleArgs& a, float u, uint32_t n_all, u64 m_all, uint32_t n_keep, u64 m_keep, int (&lo)[3], int (&hi)[3]) {
+    auto before = [&](int bin) -> u64 { return bin < NB ? s.mass[bin] : m_all; };
+    auto find = [&](bool by_rank, uint32_t rank, u64 limit) -> int {
+        __syncthreads();
+        for (int i = threadIdx.x; i < NB; i += NT) {
+            const uint32_t ce = i + 1 < NB ? s.cnt[i + 1] : n_all;
+            if (by_rank ? (s.cnt[i] < rank && rank <= ce) : (s.mass[i] <= limit && limit < before(i + 1))) s.found_bin = (uint32_t)i;
+        }
+        __syncthreads();
+        return (int)s.found_bin;
+    };
+    uint32_t n = n_all;
+    u64 k_lo = m_all, k_hi = m_all;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) { lo[i] = 0; hi[i] = -1; }
+    if (a.top_k > 0 && (uint32_t)a.top_k < n) {
+        n = (uint32_t)a.top_k;
+        lo[0] = hi[0] = find(true, n, 0);
+        k_lo = before(lo[0]);
+        k_hi = before(lo[0] + 1);
+    }
+    u64 t_lo = k_lo, t_hi = k_hi;
+    if (n_keep < n) t_lo = t_hi = m_keep;
+    if (a.top_p > 0.f && a.top_p < 1.f) {
+        const u64 l_lo = (u64)((double)a.top_p * (double)k_lo), l_hi = (u64)((double)a.top_p * (double)k_hi);
+        if (l_lo < t_hi) {
+            lo[1] = find(false, 0, min(l_lo, m_all - 1));
+            hi[1] = find(false, 0, min(l_hi, m_all - 1));
+            t_lo = min(t_lo, before(lo[1]));
+            t_hi = min(t_hi, before(hi[1] + 1));
+        }
+    }
+    t_lo = max(t_lo, (u64)1 << FRAC);                         // the first entry always stays
+    t_hi = max(t_hi, t_lo);
+    const double uu = u > 0.f ? fmin((double)u, 1.0) : 0.0;
+    const u64 d_lo = (u64)(uu * (double)t_lo), d_hi = (u64)(uu * (double)t_hi);
+    lo[2] = find(false, 0, min(d_lo - min(d_lo, (u64)1), m_all - 1));
+    hi[2] = find(false, 0, min(d_hi, m_all - 1));
+}
+
+__global__ __launch_bounds__(WT) void sample_gather_kernel(const SampleArgs a) {
+    extern __shared__ uint32_t bits[];
+    __shared__ Shared<WT> s;
+    __shared__ uint32_t base;
+    const int tid = threadIdx.x, b = blockIdx.y, j0 = blockIdx.x * a.chunk, j1 = min(j0 + a.chunk, a.V);
+    const RowWs w = row_ws(a, b);
+    const float mx = row_max(a, w);
+    if (mx == -INFINITY) return;
+    const uint32_t* barred = bar_ids<WT>(a, bits, j0, j1);
+    uint32_t n_all, n_keep;
+    u64 m_all, m_keep;
+    load_hist<WT>(s, a, w, n_all, m_all, n_keep, m_keep);
+    int lo[3], hi[3];
+    border_bins<WT>(s, a, row_u(a, b), n_all, m_all, n_keep, m_keep, lo, hi);
+    if (blockIdx.x == 0 && tid == 0) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) { w.ranges[2 * i] = lo[i]; w.ranges[2 * i + 1] = hi[i]; }
+    }
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+    Scale sc;
+    sc.set(mx, row_temp(a, b), s.tab);
+    // a chunk's members wait in LDS (the histogram has been read) for one reservation in the row's list; what does not fit there either
+    // makes the count exceed GL, and the last launch then reads the row itself
+    u64* mine = s.mass1;
+    each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int j) {
+        const int bin = sc.bin(v);
+        if ((bin >= lo[0] && bin <= hi[0]) || (bin >= lo[1] && bin <= hi[1]) || (bin >= lo[2] && bin <= hi[2])) {
+            const uint32_t k = atomicAdd(&s.n_list, 1u);
+            if (k < (uint32_t)NB) mine[k] = word_of(v, j);
+        }
+    });
+    __syncthreads();
+    const uint32_t n = s.n_list;
+    if (tid == 0) base = n ? atomicAdd(w.n_list, n > (uint32_t)NB ? (uint32_t)GL + 1 : n) : 0;      // at most MAX_SPLIT of these: no overflow
+    __syncthreads();
+    if (n > (uint32_t)NB) return;
+    for (uint32_t i = tid; i < n; i += WT) if (base + i < (uint32_t)GL) w.list[base + i] = mine[i];
+}
+
+template <int NT>
+__global__ __launch_bounds__(NT) void sample_pick_kernel(const SampleArgs a) {
+    extern __shared__ uint32_t bits[];
+    __shared__ Shared<NT> s;
+    __shared__ u64 list[GL];
+    const int tid = threadIdx.x, b = blockIdx.x;
+    const RowWs w = row_ws(a, b);
+    const float mx = row_max(a, w);
+    if (mx == -INFINITY) {
+        if (tid == 0) finish(a, b, 0, 0);
+        return;
+    }
+    const float temp = row_temp(a, b), u = row_u(a, b);
+    if (tid < 32) s.tab[tid] = exp2(tid * (1.0 / 32));
+    const uint32_t nl = w.n_list[0];
+    for (uint32_t i = tid; i < min(nl, (uint32_t)GL); i += NT) list[i] = w.list[i];
+    const uint32_t* barred = bar_ids<NT>(a, bits, 0, a.V);
+    uint32_t n_all, n_keep;
+    u64 m_all, m_keep;
+    load_hist<NT>(s, a, w, n_all, m_all, n_keep, m_keep);
+    Scale sc;
+    sc.set(mx, temp, s.tab);
+    int range[6];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) range[i] = w.ranges[i];
+    choose(a, b, u, n_all, m_all, n_keep, m_keep, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
+        // the bin of this search: gathered, or the whole row is walked
+        __syncthreads();
+        for (int i = tid; i < NB; i += NT) {
+            const uint32_t ce = i + 1 < NB ? s.cnt[i + 1] : n_all;
+            const u64 me = i + 1 < NB ? s.mass[i + 1] : m_all;
+            if (by_rank ? (s.cnt[i] < rank && rank <= ce) : (s.mass[i] <= limit && limit < me)) s.found_bin = (uint32_t)i;
+        }
+        __syncthreads();
+        const int bin = (int)s.found_bin;
+        const bool have = nl <= (uint32_t)GL && ((bin >= range[0] && bin <= range[1]) || (bin >= range[2] && bin <= range[3]) || (bin >= range[4] && bin <= range[5]));
+        __syncthreads();
+        search<NT>(s, sc, [&](auto&& f) {
+            if (have) { for (uint32_t i = tid; i < nl; i += NT) f(value_of(list[i]), index_of(list[i])); }
+            else each_entry<NT, 4>(a.logits + (size_t)b * a.ld, 0, a.V, barred, f);
+        }, n_all, m_all, by_rank, rank, limit, word, at, mass);
+    });
+}
+
+// allows a kernel more than 64 KB of LDS, once per device
+template <typename K> bool allow_lds(K kernel, size_t bytes, bool (&done)[64]) {
+    if (bytes <= 65536) return true;
     int dev = 0;
     (void)hipGetDevice(&dev);
-    if (lds > 65536 && !(dev >= 0 && dev < 64 && raised[dev])) {
-        if (hipFuncSetAttribute(reinterpret_cast<const void*>(&sample_minp_kernel<NT, ROW>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
-            return ME_ERR_LAUNCH;
-        if (dev >= 0 && dev < 64) raised[dev] = true;
-    }
-    sample_minp_kernel<NT, ROW><<<B, NT, lds, st>>>(a);
-    return me_launch_status();
+    if (dev >= 0 && dev < 64 && done[dev]) return true;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != hipSuccess) return false;
+    if (dev >= 0 && dev < 64) done[dev] = true;
+    return true;
 }
 
-int sample_call(const SampleArgs& a, int B, hipStream_t st) {
-    if (a.V <= 4096) return launch<256, true>(a, B, st);
-    if (a.V <= ROW_MAX) return launch<1024, true>(a, B, st);
-    return launch<1024, false>(a, B, st);
+// chunks of a wide row: two blocks for each CU over the batch, 2048 symbols a chunk at least
+int splits_of(int B, int V) { return std::max(1, std::min(std::min(512 / std::max(B, 1), (V + 2047) / 2048), MAX_SPLIT)); }
+
+int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st) {
+    static bool big1[64] = {}, big2[64] = {};
+    if (a.V <= ONE_BLOCK) {
+        // 256 threads to 2048 symbols: fewer waves meet at each barrier
+        if (a.V <= 2048) sample_row_kernel<256><<<B, 256, sizeof(Shared<256>) + (size_t)a.V * 4, st>>>(a);
+        else {
+            const size_t lds = sizeof(Shared<1024>) + (size_t)a.V * 4;
+            if (!allow_lds(&sample_row_kernel<1024>, lds, big1)) return ME_ERR_LAUNCH;
+            sample_row_kernel<1024><<<B, 1024, lds, st>>>(a);
+        }
+        return me_launch_status();
+    }
+    a.splits = splits_of(B, a.V);
+    a.chunk = (a.V + a.splits - 1) / a.splits;
+    a.B = B;
+    if (!ws || ((uintptr_t)ws & 15) || ws_bytes < (size_t)B * row_ws_bytes(a.splits)) return ME_ERR_WORKSPACE;
+    a.ws = (char*)ws;
+    const dim3 grid(a.splits, B);
+    const size_t bits = a.n_special > 0 ? (size_t)(a.chunk + 31) / 32 * 4 : 0, all = a.n_special > 0 ? (size_t)(a.V + 31) / 32 * 4 : 0;
+    if (!allow_lds(&sample_pick_kernel<1024>, sizeof(Shared<1024>) + GL * 8 + all, big2)) return ME_ERR_LAUNCH;
+    sample_max_kernel<<<grid, WT, bits, st>>>(a);
+    sample_hist_kernel<<<grid, WT, bits, st>>>(a);
+    sample_gather_kernel<<<grid, WT, bits, st>>>(a);
+    sample_pick_kernel<1024><<<B, 1024, all, st>>>(a);
+    return me_launch_status();
 }
 
 }  // namespace
 
+size_t me_sample_ws_bytes(int B, int V) { return B > 0 && V > ONE_BLOCK && V <= ME_SAMPLE_MAX_VOCAB ? (size_t)B * row_ws_bytes(splits_of(B, V)) : 0; }
+
 extern "C" {
 
 int me_sample_minp(const float* logits, int ld, int V, const int32_t* special, int n_special, const float* temp, int top_k, float top_p,
-                   float min_p, const float* u, int64_t* out_ids, int32_t* n_choices, int B, void* stream) {
+                   float min_p, const float* u, int64_t* out_ids, int32_t* n_choices, int B, void* ws, size_t ws_bytes, void* stream) {
     me_clear_error();
     if (!logits || !temp || !u || !out_ids || (n_special > 0 && !special)) return ME_ERR_NULL;
-    if (B < 0 || V <= 0 || V > ME_SAMPLE_MAX_VOCAB || ld < V || n_special < 0 || !(min_p >= 0.f && min_p <= 1.f)) return ME_ERR_BAD_SHAPE;
+    if (B < 0 || B > 65535 || V <= 0 || V > ME_SAMPLE_MAX_VOCAB || ld < V || n_special < 0 || !(min_p >= 0.f && min_p <= 1.f)) return ME_ERR_BAD_SHAPE;
     if (B == 0) return ME_OK;
-    SampleArgs a = {logits, ld, V, special, n_special, temp, top_k, top_p, log2((double)min_p), u, out_ids, n_choices, nullptr, nullptr, nullptr, nullptr, 0, 0, 0.f, 0.f, 0.f};
-    return sample_call(a, B, (hipStream_t)stream);
+    SampleArgs a = {};
+    a.logits = logits; a.ld = ld; a.V = V; a.special = special; a.n_special = n_special; a.temp = temp; a.top_k = top_k; a.top_p = top_p;
+    a.y_min = log2((double)min_p); a.u = u; a.out = out_ids; a.choices = n_choices;
+    return sample_call(a, B, ws, ws_bytes, (hipStream_t)stream);
 }
 
 int me_sample_minp_step(const float* logits, int ld, int V, const int32_t* special, int n_special, const int64_t* prev_tok,
                         const uint8_t* is_timeshift, float* repeat_counts, float temp_note, float temp_rest, float penalty_coeff, int top_k,
                         float top_p, float min_p, const float* u_table, int u_ld, const int32_t* pos, int pos0, int64_t* out_ids,
-                        int32_t* n_choices, int B, void* stream) {
+                        int32_t* n_choices, int B, void* ws, size_t ws_bytes, void* stream) {
     me_clear_error();
     if (!logits || !prev_tok || !is_timeshift || !repeat_counts || !u_table || !pos || !out_ids || (n_special > 0 && !special)) return ME_ERR_NULL;
-    if (B < 0 || V <= 0 || V > ME_SAMPLE_MAX_VOCAB || ld < V || u_ld < B || n_special < 0 || !(min_p >= 0.f && min_p <= 1.f)) return ME_ERR_BAD_SHAPE;
+    if (B < 0 || B > 65535 || V <= 0 || V > ME_SAMPLE_MAX_VOCAB || ld < V || u_ld < B || n_special < 0 || !(min_p >= 0.f && min_p <= 1.f)) return ME_ERR_BAD_SHAPE;
     if (B == 0) return ME_OK;
-    SampleArgs a = {logits, ld, V, special, n_special, nullptr, top_k, top_p, log2((double)min_p), u_table, out_ids, n_choices, prev_tok, is_timeshift, repeat_counts,
-                    pos, pos0, u_ld, temp_note, temp_rest, penalty_coeff};
-    return sample_call(a, B, (hipStream_t)stream);
+    SampleArgs a = {};
+    a.logits = logits; a.ld = ld; a.V = V; a.special = special; a.n_special = n_special; a.top_k = top_k; a.top_p = top_p;
+    a.y_min = log2((double)min_p); a.u = u_table; a.out = out_ids; a.choices = n_choices;
+    a.prev = prev_tok; a.is_timeshift = is_timeshift; a.repeats = repeat_counts; a.pos = pos; a.pos0 = pos0; a.u_ld = u_ld;
+    a.temp_note = temp_note; a.temp_rest = temp_rest; a.penalty = penalty_coeff;
+    return sample_call(a, B, ws, ws_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -10,7 +10,7 @@ import torch
 from . import _lib
 from ._lib import (ME_BF16, ME_F16, ME_COND_CONCAT, ME_COND_NONE, ME_COND_TOKEN, ME_EPI_OUT_F32, ME_EPI_RELU,
                    ME_EPI_RELU_BWD, ME_F32, ME_TN_MAX_GROUP, ME_WS_EMBED_BWD, ME_WS_SUMSQ, ME_WS_GEMM_TN, ME_WS_GEMM_TN_GROUP, ME_WS_RGA_DGT, ME_WS_RGA_MT,
-                   ME_WS_RGA_PT, ME_WS_RELU_MASK, ME_WS_DEC_TOKEN, ME_WS_KVQ_ATTN, check)
+                   ME_WS_RGA_PT, ME_WS_RELU_MASK, ME_WS_DEC_TOKEN, ME_WS_KVQ_ATTN, ME_WS_SAMPLE, check)
 
 DTYPE_CODE = {torch.float32: ME_F32, torch.bfloat16: ME_BF16, torch.float16: ME_F16}
 
@@ -454,21 +454,31 @@ def sample_step(logits, V, special, prev_tok, is_timeshift, repeat_counts, temp_
                                _ptr(n_choices), B, _stream()), "me_sample_step")
 
 
+def _sample_ws(B, V, device):
+    """workspace of a sampling call over wide rows: from the caching allocator, so calls on two streams or in two graphs never share one"""
+    if V <= _lib.ME_SAMPLE_ONE_BLOCK:
+        return None
+    return torch.empty(lib().me_workspace_bytes(ME_WS_SAMPLE, B, V, 0, 0), dtype=torch.uint8, device=device)
+
+
 def sample_minp(logits, V, special, temp, top_k, top_p, min_p, u, out_ids, n_choices=None):
     """one token per row of f32 logits [B, >= V] under temperature, top-k, top-p and min-p at the uniforms u (me_sample_minp)"""
     B = out_ids.numel()
+    ws = _sample_ws(B, V, logits.device)
     check(lib().me_sample_minp(_ptr(logits), logits.stride(0), V, _ptr(special), special.numel() if special is not None else 0, _ptr(temp),
-                               int(top_k), float(top_p), float(min_p), _ptr(u), _ptr(out_ids), _ptr(n_choices), B, _stream()), "me_sample_minp")
+                               int(top_k), float(top_p), float(min_p), _ptr(u), _ptr(out_ids), _ptr(n_choices), B, _ptr(ws), ws.numel() if ws is not None else 0, _stream()), "me_sample_minp")
 
 
 def sample_minp_step(logits, V, special, prev_tok, is_timeshift, repeat_counts, temp_note, temp_rest, penalty_coeff, top_k, top_p, min_p,
                      u_table, pos, pos0, out_ids, n_choices=None):
     """sample_step with min-p and for wide vocabularies (me_sample_minp_step)"""
     B = out_ids.numel()
+    ws = _sample_ws(B, V, logits.device)
     check(lib().me_sample_minp_step(_ptr(logits), logits.stride(0), V, _ptr(special), special.numel() if special is not None else 0,
                                     _ptr(prev_tok), _ptr(is_timeshift), _ptr(repeat_counts), float(temp_note), float(temp_rest),
                                     float(penalty_coeff), int(top_k), float(top_p), float(min_p), _ptr(u_table), u_table.stride(0), _ptr(pos),
-                                    int(pos0), _ptr(out_ids), _ptr(n_choices), B, _stream()), "me_sample_minp_step")
+                                    int(pos0), _ptr(out_ids), _ptr(n_choices), B, _ptr(ws), ws.numel() if ws is not None else 0, _stream()),
+          "me_sample_minp_step")
 
 
 def decode_commit(tok, history, pos, B):
