@@ -535,7 +535,7 @@ int me_sample_step(const float* logits, int ld, int V, const int32_t* special, i
  * until it has run (NULL where that is 0).
  * me_sample_minp_step is the same for a step of a device-resident loop (arguments of me_sample_step). */
 #define ME_SAMPLE_MAX_VOCAB (1 << 18)
-#define ME_SAMPLE_ONE_BLOCK 8192       /* widest row that needs no workspace */
+#define ME_SAMPLE_ONE_BLOCK 32512      /* widest row that needs no workspace */
 int me_sample_minp(const float* logits, int ld, int V, const int32_t* special, int n_special, const float* temp, int top_k, float top_p,
                    float min_p, const float* u, int64_t* out_ids, int32_t* n_choices, int B, void* ws, size_t ws_bytes, void* stream);
 int me_sample_minp_step(const float* logits, int ld, int V, const int32_t* special, int n_special, const int64_t* prev_tok,

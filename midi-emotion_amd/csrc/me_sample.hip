@@ -23,7 +23,9 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int NB = 1024;                    // bins of a search level; level 0: 32 per unit of (max - x) / temperature
-constexpr int NL = 512;                     // entries of a bin that are compared with each other directly
+constexpr int NB1 = 256;                    // pieces of a bin that holds many
+constexpr int CL = 1024;                    // entries of a bin that are collected in one walk over the row
+constexpr int NL = 128;                     // entries that are compared with each other directly
 constexpr int GL = 4096;                    // gathered entries of a wide row
 constexpr int FRAC = 45;                    // weight unit 2^-45
 constexpr int ONE_BLOCK = ME_SAMPLE_ONE_BLOCK;
@@ -49,19 +51,21 @@ struct RowWs {
     u64* mass;                              // [splits][NB]
     uint32_t* cnt;                          // [splits][NB]
     u64* m_keep;                            // [MAX_SPLIT]
+    u64* m_tot;                             // [MAX_SPLIT]
     uint32_t* n_keep;                       // [MAX_SPLIT]
     float* mx;                              // [MAX_SPLIT]
     uint32_t* n_list;                       // [4]
     int* ranges;                            // [8]: the gathered bins
     u64* list;                              // [GL]
 };
-__host__ __device__ inline size_t row_ws_bytes(int splits) { return (size_t)splits * NB * 12 + MAX_SPLIT * 16 + 16 + 32 + GL * 8; }
+__host__ __device__ inline size_t row_ws_bytes(int splits) { return (size_t)splits * NB * 12 + MAX_SPLIT * 24 + 16 + 32 + GL * 8; }
 ME_DEV RowWs row_ws(const SampleArgs& a, int b) {
     char* p = a.ws + (size_t)b * row_ws_bytes(a.splits);
     RowWs w;
     w.mass = reinterpret_cast<u64*>(p); p += (size_t)a.splits * NB * 8;
     w.cnt = reinterpret_cast<uint32_t*>(p); p += (size_t)a.splits * NB * 4;
     w.m_keep = reinterpret_cast<u64*>(p); p += MAX_SPLIT * 8;
+    w.m_tot = reinterpret_cast<u64*>(p); p += MAX_SPLIT * 8;
     w.n_keep = reinterpret_cast<uint32_t*>(p); p += MAX_SPLIT * 4;
     w.mx = reinterpret_cast<float*>(p); p += MAX_SPLIT * 4;
     w.n_list = reinterpret_cast<uint32_t*>(p); p += 16;
@@ -97,6 +101,14 @@ struct Scale {
     // 32 y; equal values (two infinities too) give 0
     ME_DEV double exponent(float v) const { return v == mx ? 0.0 : ((double)v - (double)mx) * c; }
     ME_DEV int bin(float v) const { return v == mx ? 0 : (int)fminf((mx - v) * bin_c, (float)(NB - 1)); }
+    // an interval of values that holds bins lo .. hi, a little wider: bins fall with the value, and two comparisons cost a fifth of a bin
+    ME_DEV void interval(int lo, int hi, float& v_lo, float& v_hi) const {
+        const bool any = lo <= hi;
+        const float slack = 1e-5f * fabsf(mx), at = (float)lo / bin_c, to = (float)(hi + 1) / bin_c;
+        // an infinite maximum is alone in bin 0, all else lies in the last one
+        v_hi = !any ? -INFINITY : lo == 0 ? INFINITY : mx == INFINITY ? 3.402823466e38f : mx - at * 0.9999f + slack;
+        v_lo = !any || (mx == INFINITY && hi < NB - 1) ? INFINITY : hi >= NB - 1 ? -INFINITY : mx - to * 1.0001f - slack;
+    }
     // 2^(e / 32) (e <= 0) in units of 2^-45, rounded to nearest: table times the Taylor series of 2^f, |f| <= 1/64 (6 terms: below
     // 2^-48), scaled exactly, converted by adding 2^52 (the integer is then the mantissa)
     ME_DEV u64 weight(double e) const {
@@ -130,29 +142,36 @@ ME_DEV void finish(const SampleArgs& a, int b, int64_t id, int n) {       // one
     if (a.prev) { const float rc = a.repeats[b]; a.repeats[b] = n <= 2 ? rc + 1.f : floorf(rc * 0.5f); }      // generate.py:186-189
 }
 
-template <int NT> struct Shared {
+// the exponent from which entries are in the histogram: all of them with top-k, else what min-p keeps (the doubles of keeps())
+ME_DEV double floor_of(const SampleArgs& a) {
+    if (a.top_k > 0 && a.top_k < a.V) return -INFINITY;
+    const double tiny = __longlong_as_double(__double_as_longlong(-1075.0 * 32) - 1);       // the first double above it
+    return fmax(32 * a.y_min, tiny);
+}
+
+template <int NT> struct __attribute__((aligned(16))) Shared {
     double tab[32];
     uint32_t cnt[NB];                       // level 0: per bin, then entries before it
     u64 mass[NB];
-    uint32_t cnt1[NB];                      // deeper levels
-    union {
-        u64 mass1[NB];
-        struct { u64 lw[NL], lm[NL]; };     // the last bin's entries (word, weight): the level above has been read by then
-    };
-    u64 r64[NT / 64], found_mass, found_word;
+    uint32_t cnt1[NB1];                     // deeper levels
+    u64 mass1[NB1];
+    u64 lw[CL];                             // a bin's entries
+    u64 lm[NL], lc[NL];                     // the last ones: weight, cumulative weight,
+    uint32_t lr[NL];                        // rank
+    u64 r64[NT / 64], q64[NT / 64], found_mass, found_word;
     uint32_t r32[NT / 64], found_bin, found_rank, n_list;
 };
 
-template <int NT> ME_DEV u64 block_sum64(Shared<NT>& s, u64 v) {
+// three sums at once
+template <int NT> ME_DEV void block_sum3(Shared<NT>& s, uint32_t& n, u64& x, u64& y) {
 #pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    for (int o = 32; o; o >>= 1) { n += __shfl_xor(n, o); x += __shfl_xor(x, o); y += __shfl_xor(y, o); }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.r64[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) { s.r32[threadIdx.x >> 6] = n; s.r64[threadIdx.x >> 6] = x; s.q64[threadIdx.x >> 6] = y; }
     __syncthreads();
-    u64 t = 0;
+    n = 0; x = 0; y = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) t += s.r64[w];
-    return t;
+    for (int w = 0; w < NT / 64; ++w) { n += s.r32[w]; x += s.r64[w]; y += s.q64[w]; }
 }
 template <int NT> ME_DEV u64 block_max64(Shared<NT>& s, u64 v) {
 #pragma unroll
@@ -175,13 +194,14 @@ template <int NT> ME_DEV float block_max(Shared<NT>& s, float v) {
 }
 
 // per-bin counts and masses -> what lies before each bin; returns the totals
-template <int NT> ME_DEV void scan_bins(Shared<NT>& s, uint32_t* cnt, u64* mass, uint32_t& n_all, u64& m_all) {
-    constexpr int PB = NB / NT;
+template <int NT, int N> ME_DEV void scan_bins(Shared<NT>& s, uint32_t* cnt, u64* mass, uint32_t& n_all, u64& m_all) {
+    constexpr int PB = N > NT ? N / NT : 1;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const bool on = tid * PB < N;
     uint32_t c[PB], cs = 0;
     u64 m[PB], ms = 0;
 #pragma unroll
-    for (int i = 0; i < PB; ++i) { c[i] = cnt[tid * PB + i]; m[i] = mass[tid * PB + i]; cs += c[i]; ms += m[i]; }
+    for (int i = 0; i < PB; ++i) { c[i] = on ? cnt[tid * PB + i] : 0; m[i] = on ? mass[tid * PB + i] : 0; cs += c[i]; ms += m[i]; }
     uint32_t ci = cs;
     u64 mi = ms;
 #pragma unroll
@@ -206,26 +226,68 @@ template <int NT> ME_DEV void scan_bins(Shared<NT>& s, uint32_t* cnt, u64* mass,
     mb += mi - ms;
 #pragma unroll
     for (int i = 0; i < PB; ++i) {
-        cnt[tid * PB + i] = cb; mass[tid * PB + i] = mb;
+        if (on) { cnt[tid * PB + i] = cb; mass[tid * PB + i] = mb; }
         cb += c[i]; mb += m[i];
     }
     __syncthreads();
 }
 
-// the sums of all chunks' histograms, scanned; what min-p keeps
-template <int NT> ME_DEV void load_hist(Shared<NT>& s, const SampleArgs& a, const RowWs& w, uint32_t& n_all, u64& m_all, uint32_t& n_keep, u64& m_keep) {
-    for (int i = threadIdx.x; i < NB; i += NT) {
-        uint32_t c = 0;
-        u64 m = 0;
-#pragma unroll 4
-        for (int q = 0; q < a.splits; ++q) { c += w.cnt[q * NB + i]; m += w.mass[q * NB + i]; }
-        s.cnt[i] = c;
-        s.mass[i] = m;
-    }
-    n_keep = 0; m_keep = 0;
-    for (int q = 0; q < a.splits; ++q) { n_keep += w.n_keep[q]; m_keep += w.m_keep[q]; }
+// masses alone
+template <int NT> ME_DEV void scan_mass(Shared<NT>& s, u64* mass, u64& m_all) {
+    constexpr int PB = NB / NT;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    u64 m[PB], ms = 0;
+#pragma unroll
+    for (int i = 0; i < PB; ++i) { m[i] = mass[tid * PB + i]; ms += m[i]; }
+    u64 mi = ms;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(mi, o); if (lane >= o) mi += y; }
     __syncthreads();
-    scan_bins<NT>(s, s.cnt, s.mass, n_all, m_all);
+    if (lane == 63) s.r64[wid] = mi;
+    __syncthreads();
+    u64 mb = mi - ms;
+    m_all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) { if (w < wid) mb += s.r64[w]; m_all += s.r64[w]; }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) { mass[tid * PB + i] = mb; mb += m[i]; }
+    __syncthreads();
+}
+
+// the sums of all chunks' histograms, scanned; what min-p keeps, and the weight of all entries
+template <int NT> ME_DEV void load_hist(Shared<NT>& s, const SampleArgs& a, const RowWs& w, uint32_t& n_all, u64& m_all, uint32_t& n_keep, u64& m_keep, u64& m_tot) {
+    constexpr int PB = NB / NT;
+    const int lane = threadIdx.x & 63;
+    n_keep = lane < a.splits ? w.n_keep[lane] : 0;
+    m_keep = lane < a.splits ? w.m_keep[lane] : 0;
+    m_tot = lane < a.splits ? w.m_tot[lane] : 0;
+    uint32_t c[PB] = {};
+    u64 m[PB] = {};
+    for (int q0 = 0; q0 < a.splits; q0 += 4) {                // loads of four chunks in flight, no branch between them
+        uint32_t x[4][PB];
+        u64 y[4][PB];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < PB; ++i) {
+                const int at = min(q0 + q, a.splits - 1) * NB + threadIdx.x + i * NT;
+                x[q][i] = w.cnt[at];
+                y[q][i] = w.mass[at];
+            }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < PB; ++i) { c[i] += q0 + q < a.splits ? x[q][i] : 0; m[i] += q0 + q < a.splits ? y[q][i] : 0; }
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) { s.cnt[threadIdx.x + i * NT] = c[i]; s.mass[threadIdx.x + i * NT] = m[i]; }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) { n_keep += __shfl_xor(n_keep, o); m_keep += __shfl_xor(m_keep, o); m_tot += __shfl_xor(m_tot, o); }   // 16 lanes: MAX_SPLIT
+    n_keep = __shfl(n_keep, 0);
+    m_keep = __shfl(m_keep, 0);
+    m_tot = __shfl(m_tot, 0);
+    __syncthreads();
+    scan_bins<NT, NB>(s, s.cnt, s.mass, n_all, m_all);
 }
 
 // entries [j0, j1) of a row, once each: NaN -> 0, barred ids (bit j - j0) -> -inf; f(value, index)
@@ -257,53 +319,81 @@ template <int NT> ME_DEV const uint32_t* bar_ids(const SampleArgs& a, uint32_t* 
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// the search over a scanned histogram and the entries that `each` walks.  by_rank: the mass of the first `rank` entries; else the
-// first entry whose cumulative weight exceeds `limit` (its word, its rank, the mass before it).
+// the search over a scanned histogram and the entries that `each(low, high, f)` walks (values in an interval).  by_rank: the mass of the first `rank` entries; else the
+// first entry whose cumulative weight exceeds `limit` (its word, its rank, the mass before it).  The histogram holds the entries with
+// exponents from y_floor on.
 // ---------------------------------------------------------------------------------------------------------
 template <int NT, typename EACH>
-ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, uint32_t n_all, u64 m_all, bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& before) {
+ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, double y_floor, uint32_t n_all, u64 m_all, bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& before) {
     const int tid = threadIdx.x;
     uint32_t* cnt = s.cnt;
     u64* mass = s.mass;
+    int nb = NB;
     uint32_t total = n_all, c0 = 0;                           // entries and mass before the window of this level
     u64 mtotal = m_all, m0 = 0;
     u64 hi = 0, lo = 0;
     int shift = 0, level = 0, bin0 = 0;
+    uint32_t listed = 0;                                      // entries in s.lw, once the window's fit there
+    float v_lo = 0.f, v_hi = 0.f;
 #pragma clang loop unroll(disable)
     while (true) {
-        for (int i = tid; i < NB; i += NT) {
-            const uint32_t cb = c0 + cnt[i], ce = c0 + (i + 1 < NB ? cnt[i + 1] : total);
-            const u64 mb = m0 + mass[i], me = m0 + (i + 1 < NB ? mass[i + 1] : mtotal);
+        for (int i = tid; i < nb; i += NT) {
+            const uint32_t cb = c0 + cnt[i], ce = c0 + (i + 1 < nb ? cnt[i + 1] : total);
+            const u64 mb = m0 + mass[i], me = m0 + (i + 1 < nb ? mass[i + 1] : mtotal);
             if (by_rank ? (cb < rank && rank <= ce) : (mb <= limit && limit < me)) s.found_bin = (uint32_t)i;
         }
+        if (tid == 0) s.n_list = 0;
         __syncthreads();
         const int bin = (int)s.found_bin;
-        const uint32_t cb = c0 + cnt[bin], n = c0 + (bin + 1 < NB ? cnt[bin + 1] : total) - cb;
+        const uint32_t cb = c0 + cnt[bin], n = c0 + (bin + 1 < nb ? cnt[bin + 1] : total) - cb;
         const u64 mb = m0 + mass[bin];
         if (level == 0) bin0 = bin;
         else { const u64 top = hi - ((u64)bin << shift); lo = max(lo, top - (((u64)1 << shift) - 1)); hi = top; }
         c0 = cb;
         m0 = mb;
-        __syncthreads();                                      // found_bin, cnt, mass have been read
-        auto inside = [&](float v, u64 w) { return level == 0 ? sc.bin(v) == bin0 : w <= hi && w >= lo; };
-        if (n <= NL) {
-            if (tid == 0) s.n_list = 0;
-            __syncthreads();
-            each([&](float v, int j) {
+        if (level == 0) sc.interval(bin0, bin0, v_lo, v_hi);
+        auto inside = [&](float v, u64 w) { return level == 0 ? sc.bin(v) == bin0 && sc.exponent(v) >= y_floor : w <= hi && w >= lo; };
+        if (!listed && n <= CL) {
+            each(v_lo, v_hi, [&](float v, int j) {
                 const u64 w = word_of(v, j);
                 if (inside(v, w)) s.lw[atomicAdd(&s.n_list, 1u)] = w;
             });
+            listed = n;
+        }
+        __syncthreads();                                      // and found_bin, cnt, mass have been read
+        if (listed && n <= NL) {
+            if (listed > n) {                                 // the window's part of the list to its front
+                const uint32_t per = (listed + NT - 1) / NT;
+                u64 mine[CL / NT > 0 ? CL / NT : 1];
+#pragma unroll
+                for (uint32_t q = 0; q < sizeof(mine) / 8; ++q) { const uint32_t e = tid + q * NT; mine[q] = q < per && e < listed ? s.lw[e] : 0; }
+                if (tid == 0) s.n_list = 0;
+                __syncthreads();
+#pragma unroll
+                for (uint32_t q = 0; q < sizeof(mine) / 8; ++q) if (mine[q] && mine[q] <= hi && mine[q] >= lo) s.lw[atomicAdd(&s.n_list, 1u)] = mine[q];
+                __syncthreads();
+            }
+            for (uint32_t e = tid; e < n; e += NT) { const u64 m = sc.weight(sc.exponent(value_of(s.lw[e]))); s.lm[e] = m; s.lc[e] = m; s.lr[e] = 0; }
             __syncthreads();
-            for (uint32_t e = tid; e < n; e += NT) s.lm[e] = sc.weight(sc.exponent(value_of(s.lw[e])));
+            // each entry against all others: NT / NL threads share an entry, their sums are whole numbers
+            {
+                constexpr uint32_t P = NT / NL;
+                const uint32_t e = tid % NL, per = (n + P - 1) / P, k0 = (tid / NL) * per, k1 = min(k0 + per, n);
+                if (e < n && k0 < k1) {
+                    const u64 me = s.lw[e];
+                    uint32_t r = 0;
+                    u64 cum = 0;
+#pragma clang loop unroll_count(4)
+                    for (uint32_t k = k0; k < k1; ++k) { const bool ahead = s.lw[k] > me; r += ahead; cum += ahead ? s.lm[k] : 0; }
+                    if (r) { atomicAdd(&s.lr[e], r); atomicAdd(&s.lc[e], cum); }
+                }
+            }
             __syncthreads();
             for (uint32_t e = tid; e < n; e += NT) {
-                const u64 me = s.lw[e], own = s.lm[e];
-                uint32_t r = 0;
-                u64 cum = own;
-#pragma clang loop unroll_count(4)
-                for (uint32_t k = 0; k < n; ++k) { const bool ahead = s.lw[k] > me; r += ahead; cum += ahead ? s.lm[k] : 0; }
-                const bool hit = by_rank ? c0 + r + 1 == rank : (m0 + cum > limit && m0 + cum - own <= limit);
-                if (hit) { s.found_word = me; s.found_rank = c0 + r; s.found_mass = by_rank ? m0 + cum : m0 + cum - own; }
+                const u64 cum = m0 + s.lc[e], own = s.lm[e];
+                const uint32_t r = c0 + s.lr[e];
+                const bool hit = by_rank ? r + 1 == rank : (cum > limit && cum - own <= limit);
+                if (hit) { s.found_word = s.lw[e]; s.found_rank = r; s.found_mass = by_rank ? cum : cum - own; }
             }
             __syncthreads();
             word = s.found_word;
@@ -312,38 +402,43 @@ ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, uint32_t n_all, 
             __syncthreads();
             return;
         }
-        // too many for that: the entries between the bin's first and last word, cut into 1024 pieces of the word's range (words
-        // differ, so a few levels end at one entry each)
+        // too many for that: the words between the window's first and last, cut into 256 pieces of their range (words differ, so a
+        // few levels end at one entry each); from the list where the window fits there, else from the row
+        auto window = [&](auto&& f) {
+            if (listed) { for (uint32_t e = tid; e < listed; e += NT) { const u64 w = s.lw[e]; const float v = value_of(w); if (inside(v, w)) f(w); } }
+            else each(v_lo, v_hi, [&](float v, int j) { const u64 w = word_of(v, j); if (inside(v, w)) f(w); });
+        };
         u64 wmax = 0, wmin = 0;                               // wmin as the maximum of the complement
-        each([&](float v, int j) { const u64 w = word_of(v, j); if (inside(v, w)) { wmax = max(wmax, w); wmin = max(wmin, ~w); } });
-        hi = block_max64(s, wmax);
-        lo = ~block_max64(s, wmin);
-        level = 1;
-        shift = 0;
-        while (((hi - lo) >> shift) >= NB) ++shift;
-        for (int i = tid; i < NB; i += NT) { s.cnt1[i] = 0; s.mass1[i] = 0; }
-        __syncthreads();
-        each([&](float v, int j) {
-            const u64 w = word_of(v, j);
-            if (w <= hi && w >= lo) {
-                const int i = (int)((hi - w) >> shift);
-                const u64 m = sc.weight(sc.exponent(v));
-                atomicAdd(&s.cnt1[i], 1u);
-                if (m) atomicAdd(&s.mass1[i], m);
-            }
+        window([&](u64 w) { wmax = max(wmax, w); wmin = max(wmin, ~w); });
+        for (int i = tid; i < NB1; i += NT) { s.cnt1[i] = 0; s.mass1[i] = 0; }
+        wmax = block_max64(s, wmax);
+        wmin = ~block_max64(s, wmin);
+        const int width = 64 - (int)__builtin_clzll((wmax - wmin) | 1);
+        const int next = max(0, width - 8);                   // 2^8 = NB1 pieces
+        window([&](u64 w) {
+            const int i = (int)((wmax - w) >> next);
+            const u64 m = sc.weight(sc.exponent(value_of(w)));
+            atomicAdd(&s.cnt1[i], 1u);
+            if (m) atomicAdd(&s.mass1[i], m);
         });
         __syncthreads();
+        hi = wmax;
+        lo = wmin;
+        shift = next;
+        level = 1;
         cnt = s.cnt1;
         mass = s.mass1;
-        scan_bins<NT>(s, cnt, mass, total, mtotal);
+        nb = NB1;
+        scan_bins<NT, NB1>(s, cnt, mass, total, mtotal);
     }
 }
 
-// ---- top-k, then min-p, then the nucleus, then the draw.  searcher(by_rank, rank, limit, word, at, mass)
+// ---- top-k, then min-p, then the nucleus, then the draw.  n_keep, m_keep: what min-p leaves (with top-k: of the entries in bins up to
+//      its border's); m_tot: the weight of all entries (read where top-k does not cut).  searcher(by_rank, rank, limit, word, at, mass)
 template <typename S>
-ME_DEV void choose(const SampleArgs& a, int b, float u, uint32_t n_all, u64 m_all, uint32_t n_keep, u64 m_keep, S&& searcher) {
-    u64 word = 0, mass = 0, tot = m_all, tot_k = m_all, limit = 0;
-    uint32_t at = 0, n = n_all;
+ME_DEV void choose(const SampleArgs& a, int b, float u, uint32_t n_keep, u64 m_keep, u64 m_tot, S&& searcher) {
+    u64 word = 0, mass = 0, tot = m_tot, tot_k = m_tot, limit = 0;
+    uint32_t at = 0, n = (uint32_t)a.V;
 #pragma clang loop unroll(disable)
     for (int phase = 0; phase < 3; ++phase) {
         if (phase == 0) {
@@ -384,13 +479,16 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
 #pragma unroll
         for (int q = 0; q < L; ++q) if (j0 + q * NT < V) row[j0 + q * NT] = x[q] != x[q] ? 0.f : x[q];
     }
+    const int V4 = (V + 3) / 4;                               // filled up with entries of weight 0 behind all others
+    if (tid < 4 * V4 - V) row[V + tid] = -INFINITY;
     if (tid < 32) s.tab[tid] = exp2(tid * (1.0 / 32));
     for (int i = tid; i < NB; i += NT) { s.cnt[i] = 0; s.mass[i] = 0; }
     __syncthreads();
     for (int i = tid; i < a.n_special; i += NT) { const int j = a.special[i]; if (j >= 0 && j < V) row[j] = -INFINITY; }
     __syncthreads();
+    const f32x4_t* row4 = reinterpret_cast<const f32x4_t*>(row);
     float mx = -INFINITY;
-    for (int j = tid; j < V; j += NT) mx = fmaxf(mx, row[j]);
+    for (int i = tid; i < V4; i += NT) { const f32x4_t x = row4[i]; mx = fmaxf(fmaxf(mx, fmaxf(x[0], x[1])), fmaxf(x[2], x[3])); }
     mx = block_max<NT>(s, mx);
     if (mx == -INFINITY) {                                    // nothing to choose from
         if (tid == 0) finish(a, b, 0, 0);
@@ -398,24 +496,63 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     }
     Scale sc;
     sc.set(mx, temp, s.tab);
-    auto each = [&](auto&& f) { each_entry<NT, 4>(row, 0, V, nullptr, f); };
+    auto each = [&](float low, float high, auto&& f) {
+        for (int i = tid; i < V4; i += NT) {
+            const f32x4_t x = row4[i];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (x[q] >= low && x[q] <= high) f(x[q], 4 * i + q);
+                __builtin_amdgcn_sched_barrier(0);            // the entries' f64 chains stay apart (the waves hide them): few registers
+            }
+        }
+    };
     uint32_t n_keep = 0, n_all;
-    u64 m_keep = 0, m_all;
-    each([&](float v, int) {
-        const double e = sc.exponent(v);
-        const u64 w = sc.weight(e);
-        const bool keep = Scale::keeps(e, a.y_min);
-        n_keep += keep;
-        m_keep += keep ? w : 0;
-        const int bin = sc.bin(v);
-        atomicAdd(&s.cnt[bin], 1u);
-        if (w) atomicAdd(&s.mass[bin], w);
-    });
-    n_keep = (uint32_t)block_sum64(s, (u64)n_keep);
-    m_keep = block_sum64(s, m_keep);
-    scan_bins<NT>(s, s.cnt, s.mass, n_all, m_all);
-    choose(a, b, u, n_all, m_all, n_keep, m_keep, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
-        search<NT>(s, sc, each, n_all, m_all, by_rank, rank, limit, word, at, mass);
+    u64 m_keep = 0, m_tot = 0, m_all;
+    const bool cut = a.top_k > 0 && a.top_k < V, nucleus = a.top_p > 0.f && a.top_p < 1.f;
+    float v_lo, v_hi;
+    if (cut) {
+        // counts of all entries; only those in bins up to the one that holds rank top_k can be kept, and only they get a weight
+        each(-INFINITY, INFINITY, [&](float v, int) { atomicAdd(&s.cnt[sc.bin(v)], 1u); });
+        __syncthreads();
+        scan_bins<NT, NB>(s, s.cnt, s.mass, n_all, m_all);
+        for (int i = tid; i < NB; i += NT) if (s.cnt[i] < (uint32_t)a.top_k && (uint32_t)a.top_k <= (i + 1 < NB ? s.cnt[i + 1] : n_all)) s.found_bin = (uint32_t)i;
+        __syncthreads();
+        const int bin_k = (int)s.found_bin;
+        sc.interval(0, bin_k, v_lo, v_hi);
+        each(v_lo, v_hi, [&](float v, int) {
+            const int bin = sc.bin(v);
+            if (bin > bin_k) return;
+            const double e = sc.exponent(v);
+            const u64 w = sc.weight(e);
+            const bool keep = Scale::keeps(e, a.y_min);
+            n_keep += keep;
+            m_keep += keep ? w : 0;
+            if (w) atomicAdd(&s.mass[bin], w);
+        });
+        __syncthreads();
+        scan_mass<NT>(s, s.mass, m_all);                      // the counts are scanned already
+    } else {
+        // without top-k what min-p drops is only read for the sum that the nucleus refers to
+        v_lo = nucleus || mx == INFINITY ? -INFINITY : (float)fmax((double)mx + floor_of(a) / sc.c * 1.0001 - 1e-5 * fabs((double)mx), -3.402823466e38);
+        each(v_lo, INFINITY, [&](float v, int) {
+            const double e = sc.exponent(v);
+            const bool keep = Scale::keeps(e, a.y_min);
+            if (!keep && !nucleus) return;
+            const u64 w = sc.weight(e);
+            m_tot += w;
+            if (!keep) return;
+            n_keep += 1;
+            m_keep += w;
+            const int bin = sc.bin(v);
+            atomicAdd(&s.cnt[bin], 1u);
+            if (w) atomicAdd(&s.mass[bin], w);
+        });
+        __syncthreads();
+        scan_bins<NT, NB>(s, s.cnt, s.mass, n_all, m_all);
+    }
+    block_sum3(s, n_keep, m_keep, m_tot);
+    choose(a, b, u, n_keep, m_keep, m_tot, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
+        search<NT>(s, sc, each, floor_of(a), n_all, m_all, by_rank, rank, limit, word, at, mass);
     });
 }
 
@@ -423,6 +560,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
 // wider rows: grid (splits, B) blocks of a chunk each
 // ---------------------------------------------------------------------------------------------------------
 constexpr int WT = 512;                                       // threads of a chunk's block
+constexpr int PT = 256;                                       // and of the block that finishes a row
 
 __global__ __launch_bounds__(WT) void sample_max_kernel(const SampleArgs a) {
     extern __shared__ uint32_t bits[];
@@ -443,9 +581,8 @@ __global__ __launch_bounds__(WT) void sample_max_kernel(const SampleArgs a) {
     }
 }
 ME_DEV float row_max(const SampleArgs& a, const RowWs& w) {
-    float mx = -INFINITY;
-    for (int q = 0; q < a.splits; ++q) mx = fmaxf(mx, w.mx[q]);
-    return mx;
+    const int lane = threadIdx.x & 63;
+    return wave_max(lane < a.splits ? w.mx[lane] : -INFINITY);
 }
 
 __global__ __launch_bounds__(WT) void sample_hist_kernel(const SampleArgs a) {
@@ -462,26 +599,29 @@ __global__ __launch_bounds__(WT) void sample_hist_kernel(const SampleArgs a) {
     sc.set(mx, row_temp(a, b), s.tab);
     __syncthreads();
     uint32_t n_keep = 0;
-    u64 m_keep = 0;
+    u64 m_keep = 0, m_tot = 0;
+    const bool cut = a.top_k > 0 && a.top_k < a.V, nucleus = a.top_p > 0.f && a.top_p < 1.f;
     each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int) {
         const double e = sc.exponent(v);
-        const u64 m = sc.weight(e);
         const bool keep = Scale::keeps(e, a.y_min);
+        if (!keep && !nucleus && !cut) return;
+        const u64 m = sc.weight(e);
+        m_tot += m;
         n_keep += keep;
         m_keep += keep ? m : 0;
+        if (!keep && !cut) return;                            // without top-k the histogram holds what min-p keeps
         const int bin = sc.bin(v);
         atomicAdd(&s.cnt[bin], 1u);
         if (m) atomicAdd(&s.mass[bin], m);
     });
-    n_keep = (uint32_t)block_sum64(s, (u64)n_keep);
-    m_keep = block_sum64(s, m_keep);
-    if (tid == 0) { w.n_keep[blockIdx.x] = n_keep; w.m_keep[blockIdx.x] = m_keep; }
+    block_sum3(s, n_keep, m_keep, m_tot);
+    if (tid == 0) { w.n_keep[blockIdx.x] = n_keep; w.m_keep[blockIdx.x] = m_keep; w.m_tot[blockIdx.x] = m_tot; }
     for (int i = tid; i < NB; i += WT) { w.cnt[blockIdx.x * NB + i] = s.cnt[i]; w.mass[blockIdx.x * NB + i] = s.mass[i]; }
 }
 
 // the bins that can hold a border, from the histogram alone: each search ends in a known bin, and the mass inside the
 // bins of the earlier searches bounds the limits of the later ones.  Up to three ranges of bins.
-template <int NT> ME_DEV void border_bins(Shared<NT>& s, const SampleArgs& a, float u, uint32_t n_all, u64 m_all, uint32_t n_keep, u64 m_keep, int (&lo)[3], int (&hi)[3]) {
+template <int NT> ME_DEV void border_bins(Shared<NT>& s, const SampleArgs& a, float u, uint32_t n_all, u64 m_all, uint32_t n_keep, u64 m_keep, u64 m_tot, int (&lo)[3], int (&hi)[3]) {
     auto before = [&](int bin) -> u64 { return bin < NB ? s.mass[bin] : m_all; };
     auto find = [&](bool by_rank, uint32_t rank, u64 limit) -> int {
         __syncthreads();
@@ -492,8 +632,8 @@ template <int NT> ME_DEV void border_bins(Shared<NT>& s, const SampleArgs& a, fl
         __syncthreads();
         return (int)s.found_bin;
     };
-    uint32_t n = n_all;
-    u64 k_lo = m_all, k_hi = m_all;
+    uint32_t n = (uint32_t)a.V;
+    u64 k_lo = m_tot, k_hi = m_tot;
 #pragma unroll
     for (int i = 0; i < 3; ++i) { lo[i] = 0; hi[i] = -1; }
     if (a.top_k > 0 && (uint32_t)a.top_k < n) {
@@ -531,10 +671,10 @@ __global__ __launch_bounds__(WT) void sample_gather_kernel(const SampleArgs a) {
     if (mx == -INFINITY) return;
     const uint32_t* barred = bar_ids<WT>(a, bits, j0, j1);
     uint32_t n_all, n_keep;
-    u64 m_all, m_keep;
-    load_hist<WT>(s, a, w, n_all, m_all, n_keep, m_keep);
+    u64 m_all, m_keep, m_tot;
+    load_hist<WT>(s, a, w, n_all, m_all, n_keep, m_keep, m_tot);
     int lo[3], hi[3];
-    border_bins<WT>(s, a, row_u(a, b), n_all, m_all, n_keep, m_keep, lo, hi);
+    border_bins<WT>(s, a, row_u(a, b), n_all, m_all, n_keep, m_keep, m_tot, lo, hi);
     if (blockIdx.x == 0 && tid == 0) {
 #pragma unroll
         for (int i = 0; i < 3; ++i) { w.ranges[2 * i] = lo[i]; w.ranges[2 * i + 1] = hi[i]; }
@@ -543,21 +683,23 @@ __global__ __launch_bounds__(WT) void sample_gather_kernel(const SampleArgs a) {
     __syncthreads();
     Scale sc;
     sc.set(mx, row_temp(a, b), s.tab);
-    // a chunk's members wait in LDS (the histogram has been read) for one reservation in the row's list; what does not fit there either
+    // a chunk's members wait in LDS for one reservation in the row's list; what does not fit there either
     // makes the count exceed GL, and the last launch then reads the row itself
-    u64* mine = s.mass1;
+    u64* mine = s.lw;
+    float v_lo[3], v_hi[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sc.interval(lo[i], hi[i], v_lo[i], v_hi[i]);
     each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int j) {
-        const int bin = sc.bin(v);
-        if ((bin >= lo[0] && bin <= hi[0]) || (bin >= lo[1] && bin <= hi[1]) || (bin >= lo[2] && bin <= hi[2])) {
+        if ((v >= v_lo[0] && v <= v_hi[0]) || (v >= v_lo[1] && v <= v_hi[1]) || (v >= v_lo[2] && v <= v_hi[2])) {
             const uint32_t k = atomicAdd(&s.n_list, 1u);
-            if (k < (uint32_t)NB) mine[k] = word_of(v, j);
+            if (k < (uint32_t)CL) mine[k] = word_of(v, j);
         }
     });
     __syncthreads();
     const uint32_t n = s.n_list;
-    if (tid == 0) base = n ? atomicAdd(w.n_list, n > (uint32_t)NB ? (uint32_t)GL + 1 : n) : 0;      // at most MAX_SPLIT of these: no overflow
+    if (tid == 0) base = n ? atomicAdd(w.n_list, n > (uint32_t)CL ? (uint32_t)GL + 1 : n) : 0;      // at most MAX_SPLIT of these: no overflow
     __syncthreads();
-    if (n > (uint32_t)NB) return;
+    if (n > (uint32_t)CL) return;
     for (uint32_t i = tid; i < n; i += WT) if (base + i < (uint32_t)GL) w.list[base + i] = mine[i];
 }
 
@@ -579,14 +721,14 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(const SampleArgs a) {
     for (uint32_t i = tid; i < min(nl, (uint32_t)GL); i += NT) list[i] = w.list[i];
     const uint32_t* barred = bar_ids<NT>(a, bits, 0, a.V);
     uint32_t n_all, n_keep;
-    u64 m_all, m_keep;
-    load_hist<NT>(s, a, w, n_all, m_all, n_keep, m_keep);
+    u64 m_all, m_keep, m_tot;
+    load_hist<NT>(s, a, w, n_all, m_all, n_keep, m_keep, m_tot);
     Scale sc;
     sc.set(mx, temp, s.tab);
     int range[6];
 #pragma unroll
     for (int i = 0; i < 6; ++i) range[i] = w.ranges[i];
-    choose(a, b, u, n_all, m_all, n_keep, m_keep, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
+    choose(a, b, u, n_keep, m_keep, m_tot, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
         // the bin of this search: gathered, or the whole row is walked
         __syncthreads();
         for (int i = tid; i < NB; i += NT) {
@@ -598,20 +740,20 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(const SampleArgs a) {
         const int bin = (int)s.found_bin;
         const bool have = nl <= (uint32_t)GL && ((bin >= range[0] && bin <= range[1]) || (bin >= range[2] && bin <= range[3]) || (bin >= range[4] && bin <= range[5]));
         __syncthreads();
-        search<NT>(s, sc, [&](auto&& f) {
-            if (have) { for (uint32_t i = tid; i < nl; i += NT) f(value_of(list[i]), index_of(list[i])); }
-            else each_entry<NT, 4>(a.logits + (size_t)b * a.ld, 0, a.V, barred, f);
-        }, n_all, m_all, by_rank, rank, limit, word, at, mass);
+        search<NT>(s, sc, [&](float low, float high, auto&& f) {
+            if (have) { for (uint32_t i = tid; i < nl; i += NT) { const float v = value_of(list[i]); if (v >= low && v <= high) f(v, index_of(list[i])); } }
+            else each_entry<NT, 4>(a.logits + (size_t)b * a.ld, 0, a.V, barred, [&](float v, int j) { if (v >= low && v <= high) f(v, j); });
+        }, floor_of(a), n_all, m_all, by_rank, rank, limit, word, at, mass);
     });
 }
 
 // allows a kernel more than 64 KB of LDS, once per device
-template <typename K> bool allow_lds(K kernel, size_t bytes, bool (&done)[64]) {
+template <typename K> bool allow_lds(K kernel, size_t bytes, size_t fixed, bool (&done)[64]) {
     if (bytes <= 65536) return true;
     int dev = 0;
     (void)hipGetDevice(&dev);
     if (dev >= 0 && dev < 64 && done[dev]) return true;
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != hipSuccess) return false;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - (int)fixed) != hipSuccess) return false;
     if (dev >= 0 && dev < 64) done[dev] = true;
     return true;
 }
@@ -623,10 +765,10 @@ int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st)
     static bool big1[64] = {}, big2[64] = {};
     if (a.V <= ONE_BLOCK) {
         // 256 threads to 2048 symbols: fewer waves meet at each barrier
-        if (a.V <= 2048) sample_row_kernel<256><<<B, 256, sizeof(Shared<256>) + (size_t)a.V * 4, st>>>(a);
+        if (a.V <= 2048) sample_row_kernel<256><<<B, 256, sizeof(Shared<256>) + (size_t)(a.V + 3) / 4 * 16, st>>>(a);
         else {
-            const size_t lds = sizeof(Shared<1024>) + (size_t)a.V * 4;
-            if (!allow_lds(&sample_row_kernel<1024>, lds, big1)) return ME_ERR_LAUNCH;
+            const size_t lds = sizeof(Shared<1024>) + (size_t)(a.V + 3) / 4 * 16;
+            if (!allow_lds(&sample_row_kernel<1024>, lds, 0, big1)) return ME_ERR_LAUNCH;
             sample_row_kernel<1024><<<B, 1024, lds, st>>>(a);
         }
         return me_launch_status();
@@ -638,11 +780,11 @@ int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st)
     a.ws = (char*)ws;
     const dim3 grid(a.splits, B);
     const size_t bits = a.n_special > 0 ? (size_t)(a.chunk + 31) / 32 * 4 : 0, all = a.n_special > 0 ? (size_t)(a.V + 31) / 32 * 4 : 0;
-    if (!allow_lds(&sample_pick_kernel<1024>, sizeof(Shared<1024>) + GL * 8 + all, big2)) return ME_ERR_LAUNCH;
+    if (!allow_lds(&sample_pick_kernel<PT>, sizeof(Shared<PT>) + GL * 8 + all, sizeof(Shared<PT>) + GL * 8 + 64, big2)) return ME_ERR_LAUNCH;
     sample_max_kernel<<<grid, WT, bits, st>>>(a);
     sample_hist_kernel<<<grid, WT, bits, st>>>(a);
     sample_gather_kernel<<<grid, WT, bits, st>>>(a);
-    sample_pick_kernel<1024><<<B, 1024, all, st>>>(a);
+    sample_pick_kernel<PT><<<B, PT, all, st>>>(a);
     return me_launch_status();
 }
 

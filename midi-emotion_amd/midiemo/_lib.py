@@ -17,7 +17,7 @@ ME_TN_MAX_GROUP = 5
 ABI_VERSION = 25
 ME_LO8 = 0x100             # OR-ed into the dtype of me_resid_ln_fwd / me_embed_fwd: 8-bit low halves of the residual stream
 ME_DEC_MAX_LAYERS, ME_DEC_TOKEN_ROWS = 16, 4
-ME_SAMPLE_MAX_VOCAB, ME_SAMPLE_ONE_BLOCK = 1 << 18, 8192
+ME_SAMPLE_MAX_VOCAB, ME_SAMPLE_ONE_BLOCK = 1 << 18, 32512
 # words of the loss-scaler state (me_scaler_step; enum ME_SCALER_* of include/midiemo.h)
 ME_SCALER_SCALE, ME_SCALER_INV, ME_SCALER_TRACKER, ME_SCALER_STEP, ME_SCALER_FOUND_INF, ME_SCALER_SKIPPED, ME_SCALER_WORDS = 0, 1, 2, 3, 4, 5, 8
 

@@ -20,7 +20,7 @@ def test_refusals():
         assert row(**bad) == SHAPE, bad
     assert row(B=0) == 0 and row(B=70000) == SHAPE
     need = _lib.load().me_workspace_bytes(_lib.ME_WS_SAMPLE, 3, 50000, 0, 0)
-    assert need > 0 and _lib.load().me_workspace_bytes(_lib.ME_WS_SAMPLE, 3, 8192, 0, 0) == 0
+    assert need > 0 and _lib.load().me_workspace_bytes(_lib.ME_WS_SAMPLE, 3, 32512, 0, 0) == 0
     for bad in (dict(), dict(ws=P, ws_bytes=need - 1), dict(ws=P + 8, ws_bytes=need)):
         assert row(B=3, V=50000, ld=50000, **bad) == WS, bad
     for bad in (dict(prev=None), dict(ts=None), dict(rc=None), dict(pos=None)):
