@@ -110,9 +110,13 @@ template <int BITS, bool WIDE> ME_DEV void quantise8(const float (&x)[8], u16& s
     am = max(am, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)am, 0x141, 0xF, 0xF, true));
     const float amax = __uint_as_float(am);
     const bool fine = am < 0x7f800000u, kept = fine && amax >= 0x1p-96f;
-    const uint32_t sb = __float_as_uint(amax / TOP) & 0xffff0000u;
+    // amax / TOP, correctly rounded: a constant's rounded reciprocal and one correction (amax is far from the denormals where it counts)
+    constexpr float RT = 1.f / TOP;
+    const float q_ = amax * RT;
+    const uint32_t sb = __float_as_uint(fmaf(fmaf(-q_, TOP, amax), RT, q_)) & 0xffff0000u;
     scale = fine ? (kept ? (u16)(sb >> 16) : (u16)0) : (u16)0x7fc0;
-    const float s = kept ? __uint_as_float(sb) : 1.f, r = 1.f / s;
+    // 1 / s, correctly rounded for the 8 significant bits of a scale (all of them checked): hardware estimate and one Newton step
+    const float s = kept ? __uint_as_float(sb) : 1.f, r0 = __builtin_amdgcn_rcpf(s), r = fmaf(fmaf(-s, r0, 1.f), r0, r0);
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -123,7 +127,7 @@ template <int BITS, bool WIDE> ME_DEV void quantise8(const float (&x)[8], u16& s
             const uint32_t qb = __float_as_uint(q);
             if (rem != 0.f && !(qb & 1u)) q = __uint_as_float(((__float_as_uint(rem) ^ qb) >> 31) ? qb - 1u : qb + 1u);
         }
-        y[i] = kept ? fminf(fmaxf(q, -TOP), TOP) : 0.f;
+        y[i] = fminf(fmaxf(q, -TOP), TOP);
     }
     if (BITS == 4) {
         uint32_t c = 0;
@@ -131,12 +135,12 @@ template <int BITS, bool WIDE> ME_DEV void quantise8(const float (&x)[8], u16& s
         c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[2], y[3], 1.f, 1);
         c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[4], y[5], 1.f, 2);
         c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[6], y[7], 1.f, 3);
-        codes[0] = c;
+        codes[0] = kept ? c : 0;
         codes[1] = 0;
     } else {
         int c0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), c1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
-        codes[0] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c0, true);
-        codes[1] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], c1, true);
+        codes[0] = kept ? (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c0, true) : 0;
+        codes[1] = kept ? (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], c1, true) : 0;
     }
 }
 
@@ -184,23 +188,30 @@ __global__ __launch_bounds__(256) void kvq_write_kernel(const RowArgs a) {
     __syncthreads();
     const int d = tid >> 2, q = tid & 3;                      // 8 tokens 8 q .. 8 q + 7 of dimension d
     if (d >= DH) return;
-    const int lo = max(0, t - (j0 + 8 * q)), hi = min(8, end - (j0 + 8 * q));
-    if (lo >= hi) return;
-    uint32_t word[W], mask[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w) { word[w] = 0; mask[w] = 0; }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t c = BITS == 4 ? (vq[8 * q + i][d >> 3] >> (4 * (d & 7))) & 15u : (vq[8 * q + i][d >> 2] >> (8 * (d & 3))) & 255u;
-        const bool in = i >= lo && i < hi;
-        if (BITS == 4) { word[0] |= in ? c << (4 * i) : 0u; mask[0] |= in ? 15u << (4 * i) : 0u; }
-        else { word[W - 1 < i / 4 ? 0 : i / 4] |= in ? c << (8 * (i & 3)) : 0u; mask[W - 1 < i / 4 ? 0 : i / 4] |= in ? 255u << (8 * (i & 3)) : 0u; }
-    }
     uint32_t* p = reinterpret_cast<uint32_t*>(vb + v_byte<BITS, DH>(8 * q, d));
+    const int at = BITS == 4 ? 4 * (d & 7) : 8 * (d & 3), col = BITS == 4 ? d >> 3 : d >> 2;
+    uint32_t word[W], c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = __builtin_amdgcn_ubfe(vq[8 * q + i][col], at, BITS);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-        if (mask[w] == 0xffffffffu) p[w] = word[w];
-        else if (mask[w]) p[w] = (p[w] & ~mask[w]) | word[w];
+        word[w] = c[(8 / W) * w];
+#pragma unroll
+        for (int i = 1; i < 8 / W; ++i) word[w] |= c[(8 / W) * w + i] << (BITS * i);
+    }
+    if (t <= j0 && end >= j0 + KB) {                          // block-uniform: the call covers the block
+#pragma unroll
+        for (int w = 0; w < W; ++w) p[w] = word[w];
+        return;
+    }
+    const int lo = max(0, t - (j0 + 8 * q)), hi = min(8, end - (j0 + 8 * q));
+    if (lo >= hi) return;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const int a0 = max(lo - (8 / W) * w, 0), a1 = min(hi - (8 / W) * w, 8 / W);
+        if (a0 >= a1) continue;
+        const uint32_t mask = (a1 * BITS == 32 ? 0xffffffffu : (1u << (a1 * BITS)) - 1u) & ~((1u << (a0 * BITS)) - 1u);
+        p[w] = mask == 0xffffffffu ? word[w] : (p[w] & ~mask) | (word[w] & mask);
     }
 }
 
