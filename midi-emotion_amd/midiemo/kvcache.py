@@ -21,6 +21,10 @@ def _need(ok, what):
         raise RuntimeError("kv cache: " + what)
 
 
+def _layout(*tensors):
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+
+
 class QuantKVCache:
     """Cache of `batch` sequences, `heads` heads, at least `max_len` tokens (rounded up to blocks of 32).
 
@@ -56,71 +60,96 @@ class QuantKVCache:
         self.device = k.device
         self.nbytes = 2 * (k.numel() + 2 * k_scale.numel())
         self._index = k.device.index
-        self._rows_strides = {}                 # host stride arrays by the strides they hold
+        # layouts (shapes, strides, types, devices: never addresses) that have passed the checks, with the host stride array of rows;
+        # a decode loop makes the same calls again and again, and the checks cost more host time than the launch
+        self._seen = {}
         self.ref = ops.kvq_cache(k, k_scale, v, v_scale, head_dim, bits) if k.device.type == "cuda" else None
 
     # -------------------------------------------------------------- checks
-    def _here(self, *tensors):
-        for t in tensors:
-            _need(t is None or t.device == self.device, "a tensor is on %s, the cache on %s" % (None if t is None else t.device, self.device))
+    def _passed(self, key, check, *tensors):
+        """check(*tensors) the first time a layout comes; what it returned"""
+        if key not in self._seen:
+            for t in tensors:
+                if t is not None and t.device != self.device:
+                    _need(False, "a tensor is on %s, the cache on %s" % (t.device, self.device))
+            value = check(*tensors)
+            if len(self._seen) >= 256:
+                self._seen.clear()
+            self._seen[key] = value
+        return self._seen[key]
 
-    def _pos(self, pos, n):
+    def _pos(self, pos, n, first=0):
         if isinstance(pos, torch.Tensor):
-            _need(pos.dtype == torch.int32 and pos.is_contiguous() and pos.numel() in (1, self.batch), "a position tensor must be int32 with 1 or %d values" % self.batch)
-            self._here(pos)
-        else:
-            _need(0 <= int(pos) and int(pos) + n <= self.max_len, "positions %d..%d do not fit %d tokens" % (int(pos), int(pos) + n - 1, self.max_len))
+            if not (pos.dtype is torch.int32 and pos.is_contiguous() and pos.numel() in (1, self.batch) and pos.device == self.device):
+                _need(False, "a position tensor must be int32 with 1 or %d values on %s" % (self.batch, self.device))
+        elif not (first <= pos and pos + n <= self.max_len):
+            _need(False, "positions %d..%d do not fit %d tokens" % (pos, pos + n - 1, self.max_len))
 
-    def _rows(self, k, v, pos, lens):
+    def _lens(self, lens):
+        if lens is not None and not (lens.dtype is torch.int32 and lens.shape == (self.batch,) and lens.is_contiguous() and lens.device == self.device):
+            _need(False, "lens must be int32 [%d] on %s" % (self.batch, self.device))
+
+    def _check_rows(self, k, v):
         for x in (k, v):
             _need(x.dim() == 4 and x.shape == k.shape and x.shape[0] == self.batch and x.shape[2:] == (self.heads, self.head_dim) and x.dtype == k.dtype and
                   (x.stride(3) == 1 or x.numel() == 0), "rows must be [%d, n, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
         _need(k.shape[1] <= self.max_len, "%d rows do not fit %d tokens" % (k.shape[1], self.max_len))
-        _need(lens is None or (lens.dtype == torch.int32 and lens.shape == (self.batch,) and lens.is_contiguous()), "lens must be int32 [%d]" % self.batch)
-        self._here(k, v, lens)
-        self._pos(pos, k.shape[1])
+        return ops.kvq_strides(k, v)
+
+    def _check_new(self, q, k, v):
+        for x in (k, v):
+            _need(x.shape == (self.batch, self.heads, self.head_dim) and x.dtype == q.dtype and x.stride() == k.stride() and x.stride(2) == 1,
+                  "new rows must be [%d, %d, %d] of q's type with equal strides and the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
+        return True
+
+    def _check_attend(self, q, rel, key_pad, out):
+        _need(q.dim() == 3 and q.shape == (self.batch, self.heads, self.head_dim) and q.stride(2) == 1, "q must be [%d, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(q.shape)))
+        if rel is not None:
+            _need(rel.dim() == 2 and rel.shape[1] == self.head_dim and rel.shape[0] >= self.max_len and rel.is_contiguous() and rel.dtype == q.dtype,
+                  "rel must be a contiguous [>= %d, %d] table of q's type" % (self.max_len, self.head_dim))
+        if key_pad is not None:
+            _need(key_pad.dtype == torch.uint8 and key_pad.dim() == 2 and key_pad.shape[0] == self.batch and key_pad.is_contiguous(),
+                  "key_pad must be contiguous uint8 or bool [%d, n]" % self.batch)
+        if out is not None:
+            _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1 and all(s != 0 or x == 1 for s, x in zip(out.stride(), out.shape)), "out must match q")
+        return True
 
     def _on(self):
         """the cache's device as the current one (nothing to do where it is)"""
-        _need(self.ref is not None, "it is on %s -- there is no CPU path" % self.device)
+        if self.ref is None:
+            _need(False, "it is on %s -- there is no CPU path" % self.device)
         return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
-
-    def _strides(self, k, v):
-        key = (k.stride(), v.stride())
-        if key not in self._rows_strides:
-            if len(self._rows_strides) > 64:
-                self._rows_strides.clear()
-            self._rows_strides[key] = ops.kvq_strides(k, v)
-        return self._rows_strides[key]
 
     # -------------------------------------------------------------- calls
     def write(self, k, v, pos, lens=None):
         """Quantise k, v [B, n, H, head_dim] (float32, bfloat16 or float16; any strides, last dimension contiguous) into positions pos .. pos + n - 1;
         with lens (int32 [B]) only the first lens[b] rows of sequence b.  Everything else in the cache stays as it was."""
-        self._rows(k, v, pos, lens)
-        if k.shape[1] == 0:
+        strides = self._passed(_layout(k, v), self._check_rows, k, v)
+        n = k.shape[1]
+        self._lens(lens)
+        self._pos(pos, n)
+        if n == 0:
             return
         with self._on():
-            ops.kvq_write(self.ref, k, v, pos, lens, self._strides(k, v))
+            ops.kvq_write(self.ref, k, v, pos, lens, strides)
 
     def read(self, pos, n, dtype=torch.float32, lens=None):
         """The rows at positions pos .. pos + n - 1 as (k, v) [B, n, H, head_dim] of `dtype`; rows from lens[b] on are zeros."""
-        k = torch.empty(self.batch, int(n), self.heads, self.head_dim, dtype=dtype, device=self.device)
+        _need(0 <= n <= self.max_len, "%r rows do not fit %d tokens" % (n, self.max_len))
+        self._lens(lens)
+        self._pos(pos, n)
+        k = torch.empty(self.batch, n, self.heads, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        self._rows(k, v, pos, lens)
         with self._on():
-            if k.shape[1] > 0:
-                ops.kvq_read(self.ref, k, v, pos, lens, self._strides(k, v))
+            if n > 0:
+                ops.kvq_read(self.ref, k, v, pos, lens, self._passed(_layout(k, v), self._check_rows, k, v))
         return k, v
 
     def append_attend(self, q, k, v, pos, rel=None, key_pad=None, out=None, nsplit=0):
         """A decode step in one launch: write the rows k, v [B, H, head_dim] at pos, then attend to the keys 0 .. pos.  k and v are of q's type with
         equal strides, their rows 16-byte aligned."""
-        for x in (k, v):
-            _need(x.shape == (self.batch, self.heads, self.head_dim) and x.dtype == q.dtype and x.stride() == k.stride() and x.stride(2) == 1,
-                  "new rows must be [%d, %d, %d] of q's type with equal strides and the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
-        self._here(k, v)
-        _need(isinstance(pos, torch.Tensor) or pos >= 0, "position %r has no row to write" % (pos,))
+        self._passed(_layout(q, k, v, None), self._check_new, q, k, v)
+        self._pos(pos, 1)
         return self.attend(q, pos, rel, key_pad, out, nsplit, (k, v))
 
     def attend(self, q, pos, rel=None, key_pad=None, out=None, nsplit=0, _rows=None):
@@ -128,29 +157,21 @@ class QuantKVCache:
 
         q [B, H, head_dim]; rel [M, head_dim] of q's type with M >= max_len (the model's relative table) or None; key_pad uint8 / bool
         [B, n], 1 = masked key.  A row without a key gives zeros.  nsplit: key ranges that run side by side (0: chosen from the sizes)."""
-        _need(q.dim() == 3 and q.shape == (self.batch, self.heads, self.head_dim) and q.stride(2) == 1, "q must be [%d, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(q.shape)))
-        if rel is not None:
-            _need(rel.dim() == 2 and rel.shape[1] == self.head_dim and rel.shape[0] >= self.max_len and rel.is_contiguous() and rel.dtype == q.dtype,
-                  "rel must be a contiguous [>= %d, %d] table of q's type" % (self.max_len, self.head_dim))
-        if key_pad is not None:
-            if key_pad.dtype == torch.bool:
-                key_pad = key_pad.view(torch.uint8)
-            _need(key_pad.dtype == torch.uint8 and key_pad.dim() == 2 and key_pad.shape[0] == self.batch and key_pad.is_contiguous(),
-                  "key_pad must be contiguous uint8 or bool [%d, n]" % self.batch)
-            _need(isinstance(pos, torch.Tensor) or key_pad.shape[1] > int(pos), "key_pad is narrower than the %d keys" % (0 if isinstance(pos, torch.Tensor) else int(pos) + 1))
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1 and all(s != 0 or x == 1 for s, x in zip(out.stride(), out.shape)), "out must match q")
-        self._here(q, rel, key_pad, out)
-        if isinstance(pos, torch.Tensor):
-            self._pos(pos, 1)
-            tokens = self.max_len
-        else:
-            _need(-1 <= int(pos) < self.max_len, "position %d does not fit %d tokens" % (int(pos), self.max_len))
-            tokens = max(int(pos) + 1, 1)
-        _need(0 <= nsplit <= 64, "nsplit must be 0..64")
+        if key_pad is not None and key_pad.dtype is torch.bool:
+            key_pad = key_pad.view(torch.uint8)
+        self._passed(_layout(q, rel, key_pad, out, None), self._check_attend, q, rel, key_pad, out)
+        self._pos(pos, 1 if isinstance(pos, torch.Tensor) or pos >= 0 else 0, -1)
+        tokens = self.max_len
+        if not isinstance(pos, torch.Tensor):
+            tokens = max(pos + 1, 1)
+            if key_pad is not None and key_pad.shape[1] <= pos:
+                _need(False, "key_pad is narrower than the %d keys" % (pos + 1))
+        if not 0 <= nsplit <= 64:
+            _need(False, "nsplit must be 0..64")
         with self._on():
-            ns = nsplit or ops.kvq_splits(self.batch, self.heads, tokens, rel is not None)
+            if out is None:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            ns = nsplit or self._splits(tokens, rel is not None)
             # the records of this call: from the caching allocator, so calls on two streams or in two captured graphs never share them
             part = torch.empty(self.batch * self.heads * ns * (self.head_dim + 4), dtype=torch.float32, device=self.device) if ns > 1 else None
             if _rows:
@@ -158,3 +179,11 @@ class QuantKVCache:
             else:
                 ops.kvq_attn(self.ref, q, out, pos, rel, key_pad, part, ns)
         return out
+
+    def _splits(self, tokens, rel):
+        key = (tokens, rel)
+        if key not in self._seen:
+            if len(self._seen) >= 256:
+                self._seen.clear()
+            self._seen[key] = ops.kvq_splits(self.batch, self.heads, tokens, rel)
+        return self._seen[key]
