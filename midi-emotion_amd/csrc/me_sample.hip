@@ -94,8 +94,11 @@ struct Scale {
     const double* tab;                      // 2^(i / 32)
     ME_DEV void set(float m, float temp, const double* t) {
         mx = m;
-        bin_c = (float)NB / 32.f / temp;
-        c = 32 * 1.4426950408889634074 / (double)temp;
+        // a temperature that is not positive counts as 0 (the largest entries alone have a weight), an infinite one as the largest number:
+        // exponents and bins stay ordered whatever the device memory holds
+        const float tp = temp > 0.f ? fminf(temp, 3.402823466e38f) : 0.f;
+        bin_c = (float)NB / 32.f / tp;
+        c = 32 * 1.4426950408889634074 / (double)tp;
         tab = t;
     }
     // 32 y; equal values (two infinities too) give 0
@@ -335,8 +338,11 @@ ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, double y_floor, 
     int shift = 0, level = 0, bin0 = 0;
     uint32_t listed = 0;                                      // entries in s.lw, once the window's fit there
     float v_lo = 0.f, v_hi = 0.f;
+    if (tid == 0) { s.found_bin = 0; s.found_rank = 0; s.found_mass = 0; s.found_word = 0xffffffffull; }     // index 0
+    __syncthreads();
+    // 8 bits of the word's range a level: 1 + 8 levels at most, and the loop ends there whatever it finds
 #pragma clang loop unroll(disable)
-    while (true) {
+    for (int turn = 0; turn < 10; ++turn) {
         for (int i = tid; i < nb; i += NT) {
             const uint32_t cb = c0 + cnt[i], ce = c0 + (i + 1 < nb ? cnt[i + 1] : total);
             const u64 mb = m0 + mass[i], me = m0 + (i + 1 < nb ? mass[i + 1] : mtotal);
@@ -353,15 +359,16 @@ ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, double y_floor, 
         m0 = mb;
         if (level == 0) sc.interval(bin0, bin0, v_lo, v_hi);
         auto inside = [&](float v, u64 w) { return level == 0 ? sc.bin(v) == bin0 && sc.exponent(v) >= y_floor : w <= hi && w >= lo; };
-        if (!listed && n <= CL) {
+        const bool collect = listed == 0 && n <= CL;
+        if (collect) {
             each(v_lo, v_hi, [&](float v, int j) {
                 const u64 w = word_of(v, j);
-                if (inside(v, w)) s.lw[atomicAdd(&s.n_list, 1u)] = w;
+                if (inside(v, w)) { const uint32_t k = atomicAdd(&s.n_list, 1u); if (k < CL) s.lw[k] = w; }
             });
-            listed = n;
         }
         __syncthreads();                                      // and found_bin, cnt, mass have been read
-        if (listed && n <= NL) {
+        if (collect) listed = min(s.n_list, (uint32_t)CL);
+        if ((collect || listed) && n <= NL) {
             if (listed > n) {                                 // the window's part of the list to its front
                 const uint32_t per = (listed + NT - 1) / NT;
                 u64 mine[CL / NT > 0 ? CL / NT : 1];
@@ -395,12 +402,7 @@ ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, double y_floor, 
                 const bool hit = by_rank ? r + 1 == rank : (cum > limit && cum - own <= limit);
                 if (hit) { s.found_word = s.lw[e]; s.found_rank = r; s.found_mass = by_rank ? cum : cum - own; }
             }
-            __syncthreads();
-            word = s.found_word;
-            at = s.found_rank;
-            before = s.found_mass;
-            __syncthreads();
-            return;
+            break;
         }
         // too many for that: the words between the window's first and last, cut into 256 pieces of their range (words differ, so a
         // few levels end at one entry each); from the list where the window fits there, else from the row
@@ -431,6 +433,11 @@ ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, double y_floor, 
         nb = NB1;
         scan_bins<NT, NB1>(s, cnt, mass, total, mtotal);
     }
+    __syncthreads();
+    word = s.found_word;
+    at = s.found_rank;
+    before = s.found_mass;
+    __syncthreads();
 }
 
 // ---- top-k, then min-p, then the nucleus, then the draw.  n_keep, m_keep: what min-p leaves (with top-k: of the entries in bins up to

@@ -136,6 +136,28 @@ def test_uniforms_at_and_beyond_their_ends():
     assert ids == [1, 1, 0, 0, 1] and n == [3] * 5
 
 
+@pytest.mark.parametrize("V", [12, 3000, 9000, 40000])
+def test_temperatures_at_and_beyond_their_ends(V):
+    """what is not positive counts as 0 (one of the largest, by u), an infinite one makes all entries alike"""
+    x = torch.randn(8, V, generator=torch.Generator().manual_seed(5))
+    x[:, 7] = x[:, 3] = 9.0
+    x[:, 5] = -math.inf
+    temp = torch.tensor([0.0, -1.0, math.nan, -math.inf, 1e-42, 1e-30, math.inf, 3e38])
+    u = torch.tensor([0.2, 0.7, 0.4, 0.9, 0.6, 0.3, 0.0, 0.5])
+    for rules in [(0, 1.0, 0.0), (0, 0.9, 0.1), (50, 1.0, 0.0), (3, 0.9, 0.5)]:
+        ids, n = sample(x, [], temp, *rules, u)
+        if rules[1] == 1.0:
+            assert ids[:6] == [3, 7, 3, 7, 7, 3] and n[:6] == [2] * 6
+        else:                                                    # the nucleus drops the second: half and half passes 0.9
+            assert ids[:6] == [3] * 6 and n[:6] == [1] * 6
+        kept = min(V - 1, rules[0] or V)
+        order = sorted(range(V), key=lambda j: (-float(x[6, j]), j))
+        if rules[1] == 1.0:
+            assert ids[6] == order[0] and n[6:] == [kept] * 2
+            order = sorted(range(V), key=lambda j: (-float(x[7, j]), j))
+            assert ids[7] == order[int(0.5 * kept)]
+
+
 def test_frequencies_follow_the_weights():
     V, B = 12, 4096
     x = torch.randn(V, generator=torch.Generator().manual_seed(4))
