@@ -87,35 +87,36 @@ ME_DEV float value_of(u64 word) {
 }
 ME_DEV int index_of(u64 word) { return (int)(0xffffffffu - (uint32_t)word); }
 
-// a row's scale: exponents y = (x - max) / temperature * log2 e, weights 2^y, bins
+// a row's scale: exponents y = (x - max) / temperature * log2 e, weights 2^y, bins.  Straight code: it runs once per entry.
 struct Scale {
     float mx, bin_c;
-    double c;                               // 32 log2 e / temperature
+    double mxd, c;                          // 32 log2 e / temperature
+    bool inf;                               // an infinite maximum: it alone has a weight (uniform)
     const double* tab;                      // 2^(i / 32)
     ME_DEV void set(float m, float temp, const double* t) {
         mx = m;
+        mxd = m;
+        inf = m == INFINITY;
         // a temperature that is not positive counts as 0 (the largest entries alone have a weight), an infinite one as the largest number:
-        // exponents and bins stay ordered whatever the device memory holds
+        // exponents and bins stay ordered whatever the device memory holds, and 0 times a factor is 0
         const float tp = temp > 0.f ? fminf(temp, 3.402823466e38f) : 0.f;
-        bin_c = (float)NB / 32.f / tp;
-        c = 32 * 1.4426950408889634074 / (double)tp;
+        bin_c = fminf((float)NB / 32.f / tp, 3.402823466e38f);
+        c = fmin(32 * 1.4426950408889634074 / (double)tp, 1e300);
         tab = t;
     }
-    // 32 y; equal values (two infinities too) give 0
-    ME_DEV double exponent(float v) const { return v == mx ? 0.0 : ((double)v - (double)mx) * c; }
-    ME_DEV int bin(float v) const { return v == mx ? 0 : (int)fminf((mx - v) * bin_c, (float)(NB - 1)); }
+    ME_DEV double exponent(float v) const { return inf ? (v == mx ? 0.0 : -INFINITY) : ((double)v - mxd) * c; }        // 32 y
+    ME_DEV int bin(float v) const { return inf ? (v == mx ? 0 : NB - 1) : (int)fminf((mx - v) * bin_c, (float)(NB - 1)); }
     // an interval of values that holds bins lo .. hi, a little wider: bins fall with the value, and two comparisons cost a fifth of a bin
     ME_DEV void interval(int lo, int hi, float& v_lo, float& v_hi) const {
         const bool any = lo <= hi;
         const float slack = 1e-5f * fabsf(mx), at = (float)lo / bin_c, to = (float)(hi + 1) / bin_c;
-        // an infinite maximum is alone in bin 0, all else lies in the last one
-        v_hi = !any ? -INFINITY : lo == 0 ? INFINITY : mx == INFINITY ? 3.402823466e38f : mx - at * 0.9999f + slack;
-        v_lo = !any || (mx == INFINITY && hi < NB - 1) ? INFINITY : hi >= NB - 1 ? -INFINITY : mx - to * 1.0001f - slack;
+        v_hi = !any ? -INFINITY : lo == 0 ? INFINITY : inf ? 3.402823466e38f : mx - at * 0.9999f + slack;
+        v_lo = !any || (inf && hi < NB - 1) ? INFINITY : hi >= NB - 1 ? -INFINITY : mx - to * 1.0001f - slack;
     }
     // 2^(e / 32) (e <= 0) in units of 2^-45, rounded to nearest: table times the Taylor series of 2^f, |f| <= 1/64 (6 terms: below
-    // 2^-48), scaled exactly, converted by adding 2^52 (the integer is then the mantissa)
+    // 2^-48), scaled exactly, converted by adding 2^52 (the integer is then the mantissa); from 2^-47 on, and for what is no number, 0
     ME_DEV u64 weight(double e) const {
-        if (!(e > -32.0 * (FRAC + 2))) return 0;
+        e = fmax(e, -32.0 * (FRAC + 2));
         const double k = rint(e), r = (e - k) * (0.693147180559945309417 / 32);
         const int n = (int)k;
         double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
@@ -123,9 +124,11 @@ struct Scale {
         const double scale = __longlong_as_double((long long)((n >> 5) + FRAC + 1023) << 52);
         return (u64)(__double_as_longlong(fma(p * tab[n & 31], scale, 0x1p52)) - __double_as_longlong(0x1p52));
     }
-    // what min-p and a positive weight leave: exp() of 64 bits is 0 from 2^-1075 on
-    ME_DEV static bool keeps(double e, double y_min) { return e >= 32 * y_min && e > -1075.0 * 32; }
 };
+// the exponent from which min-p and a positive weight keep an entry: exp() of 64 bits is 0 from 2^-1075 on
+ME_DEV double keep_floor(const SampleArgs& a) {
+    return fmax(32 * a.y_min, __longlong_as_double(__double_as_longlong(-1075.0 * 32) - 1));      // the first double above -1075 * 32
+}
 
 // temperature and uniform of a row (step form: the f32 operations of generate.py's sampling_temperature(), unfused)
 ME_DEV float row_temp(const SampleArgs& a, int b) {
@@ -145,12 +148,11 @@ ME_DEV void finish(const SampleArgs& a, int b, int64_t id, int n) {       // one
     if (a.prev) { const float rc = a.repeats[b]; a.repeats[b] = n <= 2 ? rc + 1.f : floorf(rc * 0.5f); }      // generate.py:186-189
 }
 
-// the exponent from which entries are in the histogram: all of them with top-k, else what min-p keeps (the doubles of keeps())
-ME_DEV double floor_of(const SampleArgs& a) {
-    if (a.top_k > 0 && a.top_k < a.V) return -INFINITY;
-    const double tiny = __longlong_as_double(__double_as_longlong(-1075.0 * 32) - 1);       // the first double above it
-    return fmax(32 * a.y_min, tiny);
-}
+// top-k cuts; min-p and the nucleus are in force
+ME_DEV bool cuts(const SampleArgs& a) { return a.top_k > 0 && a.top_k < a.V; }
+ME_DEV bool has_nucleus(const SampleArgs& a) { return a.top_p > 0.f && a.top_p < 1.f; }
+// the exponent from which entries are in the histogram: all of them with top-k, else what min-p keeps
+ME_DEV double floor_of(const SampleArgs& a) { return cuts(a) ? -INFINITY : keep_floor(a); }
 
 template <int NT> struct __attribute__((aligned(16))) Shared {
     double tab[32];
@@ -291,10 +293,24 @@ template <int NT> ME_DEV void load_hist(Shared<NT>& s, const SampleArgs& a, cons
     m_tot = __shfl(m_tot, 0);
     __syncthreads();
     scan_bins<NT, NB>(s, s.cnt, s.mass, n_all, m_all);
+    if (!cuts(a)) { n_keep = n_all; m_keep = m_all; m_tot += m_all; }
 }
 
-// entries [j0, j1) of a row, once each: NaN -> 0, barred ids (bit j - j0) -> -inf; f(value, index)
-template <int NT, int U, typename F> ME_DEV void each_entry(const float* lg, int j0, int j1, const uint32_t* barred, F&& f) {
+// ids that may not be picked, inside a chunk from j0 on: one bit each, looked at for entries before `end` only (they are mostly the first ids)
+struct Barred { const uint32_t* bits; int end; };
+template <int NT> ME_DEV Barred bar_ids(const SampleArgs& a, uint32_t* bits, int j0, int j1) {
+    if (a.n_special <= 0) return {nullptr, j0};               // uniform
+    for (int i = threadIdx.x; i < (j1 - j0 + 31) / 32 + 1; i += NT) bits[i] = 0;             // bits[0]: how far they go
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.n_special; i += NT) {
+        const int j = a.special[i];
+        if (j >= j0 && j < j1) { atomicOr(&bits[1 + ((j - j0) >> 5)], 1u << ((j - j0) & 31)); atomicMax(&bits[0], (uint32_t)(j - j0 + 1)); }
+    }
+    __syncthreads();
+    return {bits + 1, j0 + (int)__builtin_amdgcn_readfirstlane((int)bits[0])};
+}
+// entries [j0, j1) of a row, once each: NaN -> 0, barred ids -> -inf; f(value, index)
+template <int NT, int U, typename F> ME_DEV void each_entry(const float* lg, int j0, int j1, const Barred& barred, F&& f) {
     for (int i0 = j0 + (int)threadIdx.x; i0 < j1; i0 += NT * U) {
         float x[U];
 #pragma unroll
@@ -305,20 +321,12 @@ template <int NT, int U, typename F> ME_DEV void each_entry(const float* lg, int
             if (j < j1) {
                 float v = x[q];
                 if (v != v) v = 0.f;
-                if (barred && ((barred[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u)) v = -INFINITY;
+                if (j < barred.end && ((barred.bits[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u)) v = -INFINITY;
                 f(v, j);
             }
             __builtin_amdgcn_sched_barrier(0);                // the entries' f64 chains stay apart (the waves hide them): few registers
         }
     }
-}
-template <int NT> ME_DEV const uint32_t* bar_ids(const SampleArgs& a, uint32_t* bits, int j0, int j1) {
-    if (a.n_special <= 0) return nullptr;                     // uniform
-    for (int i = threadIdx.x; i < (j1 - j0 + 31) / 32; i += NT) bits[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.n_special; i += NT) { const int j = a.special[i]; if (j >= j0 && j < j1) atomicOr(&bits[(j - j0) >> 5], 1u << ((j - j0) & 31)); }
-    __syncthreads();
-    return bits;
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -515,9 +523,9 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     };
     uint32_t n_keep = 0, n_all;
     u64 m_keep = 0, m_tot = 0, m_all;
-    const bool cut = a.top_k > 0 && a.top_k < V, nucleus = a.top_p > 0.f && a.top_p < 1.f;
+    const double kept = keep_floor(a);
     float v_lo, v_hi;
-    if (cut) {
+    if (cuts(a)) {
         // counts of all entries; only those in bins up to the one that holds rank top_k can be kept, and only they get a weight
         each(-INFINITY, INFINITY, [&](float v, int) { atomicAdd(&s.cnt[sc.bin(v)], 1u); });
         __syncthreads();
@@ -531,33 +539,35 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
             if (bin > bin_k) return;
             const double e = sc.exponent(v);
             const u64 w = sc.weight(e);
-            const bool keep = Scale::keeps(e, a.y_min);
+            const bool keep = e >= kept;
             n_keep += keep;
             m_keep += keep ? w : 0;
-            if (w) atomicAdd(&s.mass[bin], w);
+            atomicAdd(&s.mass[bin], w);
         });
         __syncthreads();
         scan_mass<NT>(s, s.mass, m_all);                      // the counts are scanned already
+        block_sum3(s, n_keep, m_keep, m_tot);
     } else {
-        // without top-k what min-p drops is only read for the sum that the nucleus refers to
-        v_lo = nucleus || mx == INFINITY ? -INFINITY : (float)fmax((double)mx + floor_of(a) / sc.c * 1.0001 - 1e-5 * fabs((double)mx), -3.402823466e38);
+        // the histogram holds what min-p keeps; what it drops is only read for the sum that the nucleus refers to
+        const bool rest = has_nucleus(a) && a.y_min > -INFINITY;
+        v_lo = rest || sc.inf ? -INFINITY : (float)fmax((double)mx + kept / sc.c * 1.0001 - 1e-5 * fabs((double)mx), -3.402823466e38);
         each(v_lo, INFINITY, [&](float v, int) {
             const double e = sc.exponent(v);
-            const bool keep = Scale::keeps(e, a.y_min);
-            if (!keep && !nucleus) return;
             const u64 w = sc.weight(e);
-            m_tot += w;
-            if (!keep) return;
-            n_keep += 1;
-            m_keep += w;
-            const int bin = sc.bin(v);
-            atomicAdd(&s.cnt[bin], 1u);
-            if (w) atomicAdd(&s.mass[bin], w);
+            if (e >= kept) {
+                const int bin = sc.bin(v);
+                atomicAdd(&s.cnt[bin], 1u);
+                atomicAdd(&s.mass[bin], w);
+            } else if (rest) m_tot += w;
         });
         __syncthreads();
         scan_bins<NT, NB>(s, s.cnt, s.mass, n_all, m_all);
+        n_keep = 0;
+        if (rest) block_sum3(s, n_keep, m_keep, m_tot);
+        n_keep = n_all;
+        m_keep = m_all;
+        m_tot += m_all;
     }
-    block_sum3(s, n_keep, m_keep, m_tot);
     choose(a, b, u, n_keep, m_keep, m_tot, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
         search<NT>(s, sc, each, floor_of(a), n_all, m_all, by_rank, rank, limit, word, at, mass);
     });
@@ -574,7 +584,7 @@ __global__ __launch_bounds__(WT) void sample_max_kernel(const SampleArgs a) {
     __shared__ float red[WT / 64];
     const int b = blockIdx.y, j0 = blockIdx.x * a.chunk, j1 = min(j0 + a.chunk, a.V);
     const RowWs w = row_ws(a, b);
-    const uint32_t* barred = bar_ids<WT>(a, bits, j0, j1);
+    const Barred barred = bar_ids<WT>(a, bits, j0, j1);
     float mx = -INFINITY;
     each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int) { mx = fmaxf(mx, v); });
     mx = wave_max(mx);
@@ -599,7 +609,7 @@ __global__ __launch_bounds__(WT) void sample_hist_kernel(const SampleArgs a) {
     const RowWs w = row_ws(a, b);
     if (tid < 32) s.tab[tid] = exp2(tid * (1.0 / 32));
     for (int i = tid; i < NB; i += WT) { s.cnt[i] = 0; s.mass[i] = 0; }
-    const uint32_t* barred = bar_ids<WT>(a, bits, j0, j1);
+    const Barred barred = bar_ids<WT>(a, bits, j0, j1);
     const float mx = row_max(a, w);
     if (mx == -INFINITY) return;                              // the last launch sees it too
     Scale sc;
@@ -607,21 +617,35 @@ __global__ __launch_bounds__(WT) void sample_hist_kernel(const SampleArgs a) {
     __syncthreads();
     uint32_t n_keep = 0;
     u64 m_keep = 0, m_tot = 0;
-    const bool cut = a.top_k > 0 && a.top_k < a.V, nucleus = a.top_p > 0.f && a.top_p < 1.f;
-    each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int) {
-        const double e = sc.exponent(v);
-        const bool keep = Scale::keeps(e, a.y_min);
-        if (!keep && !nucleus && !cut) return;
-        const u64 m = sc.weight(e);
-        m_tot += m;
-        n_keep += keep;
-        m_keep += keep ? m : 0;
-        if (!keep && !cut) return;                            // without top-k the histogram holds what min-p keeps
-        const int bin = sc.bin(v);
-        atomicAdd(&s.cnt[bin], 1u);
-        if (m) atomicAdd(&s.mass[bin], m);
-    });
-    block_sum3(s, n_keep, m_keep, m_tot);
+    const bool minp = a.y_min > -INFINITY;
+    const double kept = keep_floor(a);
+    const float* lg = a.logits + (size_t)b * a.ld;
+    if (cuts(a)) {                                            // with top-k the histogram holds every entry
+        each_entry<WT, 8>(lg, j0, j1, barred, [&](float v, int) {
+            const double e = sc.exponent(v);
+            const u64 m = sc.weight(e);
+            const bool keep = e >= kept;
+            n_keep += keep;
+            m_keep += keep ? m : 0;
+            const int bin = sc.bin(v);
+            atomicAdd(&s.cnt[bin], 1u);
+            atomicAdd(&s.mass[bin], m);
+        });
+        block_sum3(s, n_keep, m_keep, m_tot);
+    } else {                                                  // else what min-p keeps; the rest counts for the nucleus' sum
+        const bool rest = minp && has_nucleus(a);
+        each_entry<WT, 8>(lg, j0, j1, barred, [&](float v, int) {
+            const double e = sc.exponent(v);
+            const u64 m = sc.weight(e);
+            if (e >= kept) {
+                const int bin = sc.bin(v);
+                atomicAdd(&s.cnt[bin], 1u);
+                atomicAdd(&s.mass[bin], m);
+            } else if (rest) m_tot += m;
+        });
+        if (rest) block_sum3(s, n_keep, m_keep, m_tot);
+        else __syncthreads();
+    }
     if (tid == 0) { w.n_keep[blockIdx.x] = n_keep; w.m_keep[blockIdx.x] = m_keep; w.m_tot[blockIdx.x] = m_tot; }
     for (int i = tid; i < NB; i += WT) { w.cnt[blockIdx.x * NB + i] = s.cnt[i]; w.mass[blockIdx.x * NB + i] = s.mass[i]; }
 }
@@ -676,7 +700,7 @@ __global__ __launch_bounds__(WT) void sample_gather_kernel(const SampleArgs a) {
     const RowWs w = row_ws(a, b);
     const float mx = row_max(a, w);
     if (mx == -INFINITY) return;
-    const uint32_t* barred = bar_ids<WT>(a, bits, j0, j1);
+    const Barred barred = bar_ids<WT>(a, bits, j0, j1);
     uint32_t n_all, n_keep;
     u64 m_all, m_keep, m_tot;
     load_hist<WT>(s, a, w, n_all, m_all, n_keep, m_keep, m_tot);
@@ -726,7 +750,7 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(const SampleArgs a) {
     if (tid < 32) s.tab[tid] = exp2(tid * (1.0 / 32));
     const uint32_t nl = w.n_list[0];
     for (uint32_t i = tid; i < min(nl, (uint32_t)GL); i += NT) list[i] = w.list[i];
-    const uint32_t* barred = bar_ids<NT>(a, bits, 0, a.V);
+    const Barred barred = bar_ids<NT>(a, bits, 0, a.V);
     uint32_t n_all, n_keep;
     u64 m_all, m_keep, m_tot;
     load_hist<NT>(s, a, w, n_all, m_all, n_keep, m_keep, m_tot);
@@ -786,7 +810,7 @@ int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st)
     if (!ws || ((uintptr_t)ws & 15) || ws_bytes < (size_t)B * row_ws_bytes(a.splits)) return ME_ERR_WORKSPACE;
     a.ws = (char*)ws;
     const dim3 grid(a.splits, B);
-    const size_t bits = a.n_special > 0 ? (size_t)(a.chunk + 31) / 32 * 4 : 0, all = a.n_special > 0 ? (size_t)(a.V + 31) / 32 * 4 : 0;
+    const size_t bits = a.n_special > 0 ? (size_t)(a.chunk + 31) / 32 * 4 + 4 : 0, all = a.n_special > 0 ? (size_t)(a.V + 31) / 32 * 4 + 4 : 0;
     if (!allow_lds(&sample_pick_kernel<PT>, sizeof(Shared<PT>) + GL * 8 + all, sizeof(Shared<PT>) + GL * 8 + 64, big2)) return ME_ERR_LAUNCH;
     sample_max_kernel<<<grid, WT, bits, st>>>(a);
     sample_hist_kernel<<<grid, WT, bits, st>>>(a);
