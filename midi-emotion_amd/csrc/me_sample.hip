@@ -24,11 +24,12 @@ typedef unsigned long long u64;
 
 constexpr int NB = 1024;                    // bins of a search level; level 0: 32 per unit of (max - x) / temperature
 constexpr int NB1 = 256;                    // pieces of a bin that holds many
-constexpr int CL = 1024;                    // entries of a bin that are collected in one walk over the row
+constexpr int CL = 512;                     // entries of a bin that are collected in one walk over the row
+constexpr int SL = 1024;                    // entries up to top-k's border that take the row's place
 constexpr int NL = 128;                     // entries that are compared with each other directly
 constexpr int GL = 4096;                    // gathered entries of a wide row
 constexpr int FRAC = 45;                    // weight unit 2^-45
-constexpr int ONE_BLOCK = ME_SAMPLE_ONE_BLOCK;
+constexpr int ONE_BLOCK = ME_SAMPLE_ONE_BLOCK;              // 32512: its row, the bins and the lists fill 160 KB of LDS
 constexpr int MAX_SPLIT = 16;               // chunks of a wide row at most: every later block reads all chunks' histograms
 
 struct SampleArgs {
@@ -482,7 +483,8 @@ template <int NT>
 __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     Shared<NT>& s = *reinterpret_cast<Shared<NT>*>(smem);
-    float* row = reinterpret_cast<float*>(smem + sizeof(Shared<NT>));
+    u64* head = reinterpret_cast<u64*>(smem + sizeof(Shared<NT>));                    // [SL]
+    float* row = reinterpret_cast<float*>(head + SL);
     const int tid = threadIdx.x, b = blockIdx.x, V = a.V;
     const float* lg = a.logits + (size_t)b * a.ld;
     const float temp = row_temp(a, b), u = row_u(a, b);
@@ -525,6 +527,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
     u64 m_keep = 0, m_tot = 0, m_all;
     const double kept = keep_floor(a);
     float v_lo, v_hi;
+    uint32_t n_head = 0;                                      // entries in `head`, where they hold all that can be kept
     if (cuts(a)) {
         // counts of all entries; only those in bins up to the one that holds rank top_k can be kept, and only they get a weight
         each(-INFINITY, INFINITY, [&](float v, int) { atomicAdd(&s.cnt[sc.bin(v)], 1u); });
@@ -533,17 +536,24 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
         for (int i = tid; i < NB; i += NT) if (s.cnt[i] < (uint32_t)a.top_k && (uint32_t)a.top_k <= (i + 1 < NB ? s.cnt[i + 1] : n_all)) s.found_bin = (uint32_t)i;
         __syncthreads();
         const int bin_k = (int)s.found_bin;
+        n_head = bin_k + 1 < NB ? s.cnt[bin_k + 1] : n_all;
+        if (n_head > SL) n_head = 0;
         sc.interval(0, bin_k, v_lo, v_hi);
-        each(v_lo, v_hi, [&](float v, int) {
-            const int bin = sc.bin(v);
-            if (bin > bin_k) return;
+        auto add = [&](float v, int bin) {
             const double e = sc.exponent(v);
             const u64 w = sc.weight(e);
             const bool keep = e >= kept;
             n_keep += keep;
             m_keep += keep ? w : 0;
             atomicAdd(&s.mass[bin], w);
-        });
+        };
+        if (n_head) {                                         // few: collected first, a thread each from here on
+            if (tid == 0) s.n_list = 0;
+            __syncthreads();
+            each(v_lo, v_hi, [&](float v, int j) { if (sc.bin(v) <= bin_k) head[atomicAdd(&s.n_list, 1u)] = word_of(v, j); });
+            __syncthreads();
+            for (uint32_t i = tid; i < n_head; i += NT) { const float v = value_of(head[i]); add(v, sc.bin(v)); }
+        } else each(v_lo, v_hi, [&](float v, int) { const int bin = sc.bin(v); if (bin <= bin_k) add(v, bin); });
         __syncthreads();
         scan_mass<NT>(s, s.mass, m_all);                      // the counts are scanned already
         block_sum3(s, n_keep, m_keep, m_tot);
@@ -569,7 +579,10 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
         m_tot += m_all;
     }
     choose(a, b, u, n_keep, m_keep, m_tot, [&](bool by_rank, uint32_t rank, u64 limit, u64& word, uint32_t& at, u64& mass) {
-        search<NT>(s, sc, each, floor_of(a), n_all, m_all, by_rank, rank, limit, word, at, mass);
+        search<NT>(s, sc, [&](float low, float high, auto&& f) {
+            if (n_head) { for (uint32_t i = tid; i < n_head; i += NT) { const float v = value_of(head[i]); if (v >= low && v <= high) f(v, index_of(head[i])); } }
+            else each(low, high, f);
+        }, floor_of(a), n_all, m_all, by_rank, rank, limit, word, at, mass);
     });
 }
 
@@ -696,6 +709,7 @@ __global__ __launch_bounds__(WT) void sample_gather_kernel(const SampleArgs a) {
     extern __shared__ uint32_t bits[];
     __shared__ Shared<WT> s;
     __shared__ uint32_t base;
+    __shared__ u64 mine[SL];
     const int tid = threadIdx.x, b = blockIdx.y, j0 = blockIdx.x * a.chunk, j1 = min(j0 + a.chunk, a.V);
     const RowWs w = row_ws(a, b);
     const float mx = row_max(a, w);
@@ -716,21 +730,20 @@ __global__ __launch_bounds__(WT) void sample_gather_kernel(const SampleArgs a) {
     sc.set(mx, row_temp(a, b), s.tab);
     // a chunk's members wait in LDS for one reservation in the row's list; what does not fit there either
     // makes the count exceed GL, and the last launch then reads the row itself
-    u64* mine = s.lw;
     float v_lo[3], v_hi[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) sc.interval(lo[i], hi[i], v_lo[i], v_hi[i]);
     each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int j) {
         if ((v >= v_lo[0] && v <= v_hi[0]) || (v >= v_lo[1] && v <= v_hi[1]) || (v >= v_lo[2] && v <= v_hi[2])) {
             const uint32_t k = atomicAdd(&s.n_list, 1u);
-            if (k < (uint32_t)CL) mine[k] = word_of(v, j);
+            if (k < (uint32_t)SL) mine[k] = word_of(v, j);
         }
     });
     __syncthreads();
     const uint32_t n = s.n_list;
-    if (tid == 0) base = n ? atomicAdd(w.n_list, n > (uint32_t)CL ? (uint32_t)GL + 1 : n) : 0;      // at most MAX_SPLIT of these: no overflow
+    if (tid == 0) base = n ? atomicAdd(w.n_list, n > (uint32_t)SL ? (uint32_t)GL + 1 : n) : 0;      // at most MAX_SPLIT of these: no overflow
     __syncthreads();
-    if (n > (uint32_t)CL) return;
+    if (n > (uint32_t)SL) return;
     for (uint32_t i = tid; i < n; i += WT) if (base + i < (uint32_t)GL) w.list[base + i] = mine[i];
 }
 
@@ -796,9 +809,10 @@ int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st)
     static bool big1[64] = {}, big2[64] = {};
     if (a.V <= ONE_BLOCK) {
         // 256 threads to 2048 symbols: fewer waves meet at each barrier
-        if (a.V <= 2048) sample_row_kernel<256><<<B, 256, sizeof(Shared<256>) + (size_t)(a.V + 3) / 4 * 16, st>>>(a);
+        if (a.V <= 2048) sample_row_kernel<256><<<B, 256, sizeof(Shared<256>) + SL * 8 + (size_t)(a.V + 3) / 4 * 16, st>>>(a);
         else {
-            const size_t lds = sizeof(Shared<1024>) + (size_t)(a.V + 3) / 4 * 16;
+            static_assert(sizeof(Shared<1024>) + SL * 8 + (size_t)ONE_BLOCK * 4 <= 160 * 1024, "the widest row of one block");
+            const size_t lds = sizeof(Shared<1024>) + SL * 8 + (size_t)(a.V + 3) / 4 * 16;
             if (!allow_lds(&sample_row_kernel<1024>, lds, 0, big1)) return ME_ERR_LAUNCH;
             sample_row_kernel<1024><<<B, 1024, lds, st>>>(a);
         }
