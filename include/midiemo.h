@@ -470,7 +470,7 @@ int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
  * me_kvq_attn: one query per (sequence, head), q / out: T [B][H][dh] with strides ldq_* / ldo_* (elements):
  *     out = sum_j softmax_j( (q.k_j + q.E[M-1-(t-j)]) / sqrt(dh) ) v_j   over keys j = 0 .. t that key_pad leaves (music_multi.py:211-235)
  *   E (T [M][dh] natural layout, 16-byte aligned; NULL: no relative term) needs M >= 32 * blocks.  key_pad: uint8 [B][ld_pad] or NULL,
- *   1 = masked; keys from ld_pad on are not masked.  A masked row's codes and scale are never used, whatever they hold.  No
+ *   1 = masked; keys from ld_pad on are not masked.  A query that holds an infinity or a NaN gives NaN.  A masked row's codes and scale are never used, whatever they hold.  No
  *   key left (t = -1, or all masked): zeros.  nsplit in 1 .. 64 key ranges (me_kvq_splits gives a good number; rel: with a relative table); with nsplit > 1
  *   `part` (me_workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh, dtype) bytes, 16-byte aligned, uninitialised, private to the
  *   call until it has run) holds the ranges' records and a second launch joins them in ascending order.  out = NULL: the records are the

@@ -479,11 +479,12 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
     bf16x8_t ha[4], hb[4];                                    // 8 bits: steps of 8 codes
     {
         float x = lane < DH ? qs[hh][lane] : 0.f;
+        if (__builtin_amdgcn_ballot_w64(!(fabsf(x) <= 3.402823466e38f))) { qinv = __builtin_nanf(""); x = 0.f; }   // an infinity or a NaN in the query: every logit is NaN
         if constexpr (BITS == 4) {
-            float f;
-            unit(wave_max(fabsf(x)), f, qinv);
+            float f, fi;
+            unit(wave_max(fabsf(x)), f, fi);
+            qinv *= fi;
             x *= f;
-            if (__builtin_amdgcn_ballot_w64(!(fabsf(x) < 32.f))) { qinv = __builtin_nanf(""); x = 0.f; }   // an infinity or a NaN in the query: every logit is NaN
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 const float d = rintf(x);
@@ -580,7 +581,7 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
 #pragma unroll
             for (int i = 0; i < 8; ++i) jo[wid][d0 + i] = x[i];
         }
-        s = wave_sum(s) * cs;
+        s = wave_sum(s) * cs + (qinv - qinv);                 // NaN with a query that is none
         lds_order();
         if (!(pad && t < a.ld_pad && pad[t]) && s != -INFINITY) {
             const float one = __builtin_amdgcn_exp2f(s - s);  // 1, or NaN where the logit is none
@@ -599,7 +600,7 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
         const int c1 = min(c0 + stretch, j1);
         if constexpr (REL) {
             __syncthreads();                                  // the last stretch has been read
-            constexpr int U = 4;                              // key groups of 16 in flight per wave
+            constexpr int U = BITS == 4 ? 4 : 2;              // key groups of 16 in flight per wave (8 bits: four would spill)
             for (int k0 = wid * 16; k0 < c1 - c0; k0 += nw * 16 * U) {
                 EFrag<T, DH> e[U];
 #pragma unroll

@@ -263,6 +263,20 @@ def test_append_and_attend_in_one_launch(T, dh, bits):
         assert bool(torch.isnan(out[0, 0]).all()) and bool(torch.isfinite(out[2:]).all())
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("T", ["bf16", "f16", "f32"])
+def test_a_query_that_is_no_number_gives_none(T, bits):
+    c = cache(1, 3, 40, 48, bits)
+    fill(c, 40, DT[T], 3)
+    E = torch.randn(2048, 48).to(DT[T]).cuda()
+    for bad in (math.inf, -math.inf, math.nan):
+        q = torch.randn(1, 3, 48).to(DT[T])
+        q[0, 1, 47] = bad
+        for rel in (None, E):
+            for out in (c.attend(q.cuda(), 39, rel=rel), c.append_attend(q.cuda(), q.cuda() * 0 + 1, q.cuda() * 0 + 1, 39, rel=rel)):
+                assert bool(torch.isnan(out[0, 1]).all()), bad
+
+
 def test_attention_values_that_are_not_numbers():
     c = cache(2, 2, 64, 64, 4)
     x = rows(2, 64, 2, 64, torch.bfloat16, 2)
