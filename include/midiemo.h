@@ -451,7 +451,7 @@ int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
  *   code  = x / scale to the nearest value of the code's type, ties to the even code, larger ones to the largest;
  * a row with amax < 2^-96 is held as zeros (scale 0), a row with an infinity or a NaN reads back as NaN (scale NaN, codes 0).
  * 32 tokens form a block; `blocks` of them per (sequence, head) are the cache's room:
- *   kcodes / vcodes : uint8 [B][H][blocks][32 * dh * bits / 8], 16-byte aligned, ZERO before the first use
+ *   kcodes / vcodes : uint8 [B][H][blocks][32 * dh * bits / 8], 16-byte aligned; like the scales they need no clearing
  *   kscale / vscale : bfloat16 [B][H][blocks * 32]
  * Order of the codes inside a block (position p counts codes; 4 bits: byte p / 2, low nibble first):
  *   K, 4 bits: p = (group * 16 + token % 16) * 32 + i;  dh 64: group = 2 (token / 16) + d / 32, i = d % 32;  dh 32: group = token / 16,
@@ -470,8 +470,10 @@ int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
  * me_kvq_attn: one query per (sequence, head), q / out: T [B][H][dh] with strides ldq_* / ldo_* (elements):
  *     out = sum_j softmax_j( (q.k_j + q.E[M-1-(t-j)]) / sqrt(dh) ) v_j   over keys j = 0 .. t that key_pad leaves (music_multi.py:211-235)
  *   E (T [M][dh] natural layout, 16-byte aligned; NULL: no relative term) needs M >= 32 * blocks.  key_pad: uint8 [B][ld_pad] or NULL,
- *   1 = masked; keys from ld_pad on are not masked.  A query that holds an infinity or a NaN gives NaN.  A masked row's codes and scale are never used, whatever they hold.  No
- *   key left (t = -1, or all masked): zeros.  nsplit in 1 .. 64 key ranges (me_kvq_splits gives a good number; rel: with a relative table); with nsplit > 1
+ *   1 = masked; keys from ld_pad on are not masked.  A query that holds an infinity or a NaN gives NaN.
+ *   A masked row's codes and scale, and those behind position t, do not matter, whatever they hold.  (The write leaves no code that is no
+ *   number -- e4m3 0x7f, 0xff; in a row that is attended to, such a code's effect is unspecified.)
+ *   No key left (t = -1, or all masked): zeros.  nsplit in 1 .. 64 key ranges (me_kvq_splits gives a good number; rel: with a relative table); with nsplit > 1
  *   `part` (me_workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh, dtype) bytes, 16-byte aligned, uninitialised, private to the
  *   call until it has run) holds the ranges' records and a second launch joins them in ascending order.  out = NULL: the records are the
  *   result, as me_dec_attn leaves them (nsplit <= 8: me_dec_proj_resid joins them; it takes a row without keys for NaN). */
@@ -521,7 +523,7 @@ int me_sample_step(const float* logits, int ld, int V, const int32_t* special, i
                    int top_k, float top_p, const float* u_table, int u_ld, const int32_t* pos, int pos0, int64_t* out_ids,
                    int32_t* n_choices, int B, void* stream);
 
-/* Sampling with min-p and for wide vocabularies (V <= ME_SAMPLE_MAX_VOCAB), one launch for the whole batch (four beyond 8192 symbols): the rules of
+/* Sampling with min-p and for wide vocabularies (V <= ME_SAMPLE_MAX_VOCAB), one launch for the whole batch (four for rows of more than ME_SAMPLE_ONE_BLOCK symbols): the rules of
  * me_sample_topk_topp with min-p behind them and the arithmetic in 64 bits.  NaN -> 0, ids in special[] -> -inf; entries in the order
  * (logit descending, index ascending); weight w = exp((x - max x) / temp[b]); kept are the entries that pass all of
  *   top_k  (> 0): the first top_k entries;

@@ -369,6 +369,14 @@ ME_DEV bf16x8_t widen8(uint32_t c0, uint32_t c1) {
     const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, 1.f, true);
     return (bf16x8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// e4m3 codes that are no numbers (0x7f, 0xff; never written, but memory that was never written may hold them) become zeros
+ME_DEV void numbers(u32x4_t& x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t m = ((x[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        x[i] &= ~(m - (m >> 7));
+    }
+}
 ME_DEV f32x4_t mma_bf16(const bf16x8_t& a, const bf16x8_t& b, const f32x4_t& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 ME_DEV void lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }      // a wave's own LDS writes, then its reads
 ME_DEV i32x8_t two_pieces(const u32x4_t& lo, const u32x4_t& hi) {
@@ -624,6 +632,16 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
             Tile<BITS, DH> nxt;
             const bool more = jt + kw * TK < j1;
             if (more) load_tile<BITS, DH>(nxt, kc, vc, ks, vs, pad, a.ld_pad, jt + kw * TK, j1, lane);
+            // 8 bits: a code meets the other rows' zeros in the products, so where a key of the tile is left out all codes have to be numbers
+            if (BITS == 8 && __builtin_amdgcn_ballot_w64(cur.pad[0] | cur.pad[1])) {
+#pragma unroll
+                for (int s = 0; s < Tile<BITS, DH>::P; ++s) {
+#pragma unroll
+                    for (int u = 0; u < Tile<BITS, DH>::NK; ++u) numbers(cur.k[u][s]);
+#pragma unroll
+                    for (int u = 0; u < Tile<BITS, DH>::NV; ++u) numbers(cur.v[u][s]);
+                }
+            }
             // ---- logits of keys jt + lane and jt + 64 + lane
             float s[2];
 #pragma unroll

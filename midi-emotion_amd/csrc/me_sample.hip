@@ -823,6 +823,7 @@ int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st)
     a.B = B;
     if (!ws || ((uintptr_t)ws & 15) || ws_bytes < (size_t)B * row_ws_bytes(a.splits)) return ME_ERR_WORKSPACE;
     a.ws = (char*)ws;
+    static_assert(sizeof(Shared<WT>) + SL * 8 + 16 + ME_SAMPLE_MAX_VOCAB / 8 + 8 <= 65536, "a chunk of the widest row, with its barred ids");
     const dim3 grid(a.splits, B);
     const size_t bits = a.n_special > 0 ? (size_t)(a.chunk + 31) / 32 * 4 + 4 : 0, all = a.n_special > 0 ? (size_t)(a.V + 31) / 32 * 4 + 4 : 0;
     if (!allow_lds(&sample_pick_kernel<PT>, sizeof(Shared<PT>) + GL * 8 + all, sizeof(Shared<PT>) + GL * 8 + 64, big2)) return ME_ERR_LAUNCH;

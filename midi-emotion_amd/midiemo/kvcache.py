@@ -43,7 +43,8 @@ class QuantKVCache:
 
     @classmethod
     def wrap(cls, k, k_scale, v, v_scale, head_dim, bits):
-        """A cache over existing tensors: codes uint8 [B, H, blocks, 32 * head_dim * bits / 8], scales bfloat16 [B, H, blocks * 32]."""
+        """A cache over existing tensors: codes uint8 [B, H, blocks, 32 * head_dim * bits / 8], 16-byte aligned, and
+        scales bfloat16 [B, H, blocks * 32]; none of them needs to be cleared before rows are written."""
         self = cls.__new__(cls)
         _need(head_dim in HEAD_DIMS and bits in (4, 8), "head_dim must be 32, 48 or 64 and bits 4 or 8 (got %r, %r)" % (head_dim, bits))
         _need(k.dim() == 4 and all(x > 0 for x in k.shape) and k.shape[3] == BLOCK * head_dim * bits // 8, "codes must be [B, H, blocks, %d], got %s" % (BLOCK * head_dim * bits // 8, tuple(k.shape)))
@@ -68,7 +69,8 @@ class QuantKVCache:
     # -------------------------------------------------------------- checks
     def _passed(self, key, check, *tensors):
         """check(*tensors) the first time a layout comes; what it returned"""
-        if key not in self._seen:
+        value = self._seen.get(key)
+        if value is None:
             for t in tensors:
                 if t is not None and t.device != self.device:
                     _need(False, "a tensor is on %s, the cache on %s" % (t.device, self.device))
@@ -76,7 +78,7 @@ class QuantKVCache:
             if len(self._seen) >= 256:
                 self._seen.clear()
             self._seen[key] = value
-        return self._seen[key]
+        return value
 
     def _pos(self, pos, n, first=0):
         if isinstance(pos, torch.Tensor):
@@ -182,8 +184,9 @@ class QuantKVCache:
 
     def _splits(self, tokens, rel):
         key = (tokens, rel)
-        if key not in self._seen:
+        value = self._seen.get(key)
+        if value is None:
             if len(self._seen) >= 256:
                 self._seen.clear()
-            self._seen[key] = ops.kvq_splits(self.batch, self.heads, tokens, rel)
-        return self._seen[key]
+            value = self._seen[key] = ops.kvq_splits(self.batch, self.heads, tokens, rel)
+        return value

@@ -112,3 +112,11 @@ def test_refusals_of_the_c_abi():
         for b, h, n in ((1, 8, 1), (1, 8, 2048), (4, 8, 2048), (64, 16, 1999), (1, 1, 1 << 30), (10 ** 6, 8, 2048), (0, 1, 1)):
             assert 1 <= lib.me_kvq_splits(b, h, n, rel) <= 64
     assert lib.me_kvq_splits(4, 8, 2048, 1) == 16 and lib.me_kvq_splits(4, 8, 2048, 0) == 1 and lib.me_kvq_splits(1, 1, 1 << 30, 0) == 64
+
+
+def test_layouts_once_checked_survive_a_flush_by_another_thread():
+    c = QuantKVCache(1, 1, 32, 64, 4, "cpu")
+    flush = lambda *t: c._seen.clear() or 5
+    for i in range(300):
+        assert c._passed((i, "key"), flush) == 5
+    assert len(c._seen) <= 256

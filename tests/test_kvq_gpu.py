@@ -277,6 +277,38 @@ def test_a_query_that_is_no_number_gives_none(T, bits):
                 assert bool(torch.isnan(out[0, 1]).all()), bad
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dh", [32, 48, 64])
+def test_what_unused_rows_hold_does_not_matter(dh, bits):
+    """masked rows and those behind the position: every code and scale there may be anything, numbers or not"""
+    B, H, n, pos = 3, 2, 320, 200
+    E = torch.randn(n, dh).bfloat16().cuda()
+    q = torch.randn(B, H, dh).bfloat16().cuda()
+    pad = (torch.rand(B, n) < 0.3).to(torch.uint8)
+    pad[2] = 0
+    x, y = rows(B, n, H, dh, torch.bfloat16, 5).cuda().unbind(2)[1:]
+    got = []
+    for junk in (0x00, 0x7f, 0xff, 0x5a):
+        c = cache(B, H, n, dh, bits)
+        for t in (c.k, c.v):
+            t.fill_(junk)
+        for t in (c.k_scale, c.v_scale):
+            t.view(torch.uint8).fill_(junk)
+        for j in range(pos + 1):                                 # only the rows that count are written
+            for b in range(B):
+                if not pad[b, j]:
+                    one = torch.zeros(B, dtype=torch.int32)
+                    one[b] = 1
+                    c.write(x[:, j : j + 1], y[:, j : j + 1], j, lens=one.cuda())
+        p = pad.cuda()
+        got.append([c.attend(q, pos, rel=E, key_pad=p), c.attend(q, pos, key_pad=p),
+                    c.append_attend(q, x[:, pos + 1].contiguous(), y[:, pos + 1].contiguous(), pos + 1, rel=E, key_pad=p)])
+        assert all(bool(torch.isfinite(o).all()) for o in got[-1])
+    for g in got[1:]:
+        for a, b in zip(got[0], g):
+            assert torch.equal(a, b)
+
+
 def test_attention_values_that_are_not_numbers():
     c = cache(2, 2, 64, 64, 4)
     x = rows(2, 64, 2, 64, torch.bfloat16, 2)
@@ -364,7 +396,7 @@ def test_two_streams_attend_one_cache():
 
 
 def test_offsets_beyond_32_bits():
-    """the last sequence of a cache whose codes pass 4 GiB: 40 sequences of 131072 + tokens"""
+    """the last sequence of a cache whose codes pass 4 GiB: 68 sequences of 131072 + tokens"""
     B, H, room, dh = 68, 8, 131072, 64
     c = cache(B, H, room, dh, 8)
     assert c.k.numel() > 2 ** 32

@@ -1,5 +1,8 @@
 """Refusals of me_sample_minp and me_sample_minp_step: made on the host, before anything is enqueued (addresses are never touched)."""
-from midiemo import _lib
+import pytest
+import torch
+
+from midiemo import _lib, ops
 
 P = 4096
 NULL, SHAPE, WS = -5, -2, -6
@@ -28,3 +31,22 @@ def test_refusals():
     for bad in (dict(u_ld=3, B=4), dict(V=0), dict(min_p=2.0)):
         assert step(**bad) == SHAPE, bad
     assert step(B=0) == 0
+
+
+def test_tensors_that_do_not_fit_are_refused():
+    f = lambda *s: torch.zeros(*s)
+    ids, special, counts = torch.zeros(3, dtype=torch.int64), torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    good = dict(logits=f(3, 9), V=9, special=special, temp=f(3), u=f(3), ids=ids, counts=counts)
+    for key, bad in (("logits", f(3, 9).half()), ("logits", f(2, 9)), ("logits", f(3, 8)), ("logits", f(9, 3).t()), ("logits", f(27)), ("temp", f(2)),
+                     ("temp", f(3).double()), ("u", f(6)[::2]), ("ids", counts), ("ids", torch.zeros(6, dtype=torch.int64)[::2]), ("special", ids),
+                     ("counts", ids), ("counts", special), ("u", torch.zeros(3, device="meta"))):
+        a = {**good, key: bad}
+        with pytest.raises(RuntimeError, match="sampling: "):
+            ops.sample_minp(a["logits"], a["V"], a["special"], a["temp"], 0, 0.9, 0.1, a["u"], a["ids"], a["counts"])
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.sample_minp(good["logits"], 9, special, good["temp"], 0, 0.9, 0.1, good["u"], ids, counts)
+    marks, prev, table, pos = torch.zeros(9, dtype=torch.uint8), torch.zeros(3, dtype=torch.int64), f(5, 3), torch.zeros(1, dtype=torch.int32)
+    for bad in ((prev.int(), marks, table, pos), (prev[:2], marks, table, pos), (prev, marks.bool(), table, pos), (prev, marks[:8], table, pos),
+                (prev, marks, f(5, 2), pos), (prev, marks, f(3, 5).t(), pos), (prev, marks, table, pos.long())):
+        with pytest.raises(RuntimeError, match="sampling: "):
+            ops.sample_minp_step(good["logits"], 9, special, bad[0], bad[1], f(3), 1.0, 1.0, 0.5, 0, 0.9, 0.1, bad[2], bad[3], 0, ids, counts)
