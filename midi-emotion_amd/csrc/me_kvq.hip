@@ -632,50 +632,50 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
             Tile<BITS, DH> nxt;
             const bool more = jt + kw * TK < j1;
             if (more) load_tile<BITS, DH>(nxt, kc, vc, ks, vs, pad, a.ld_pad, jt + kw * TK, j1, lane);
-            // 8 bits: a code meets the other rows' zeros in the products, so where a key of the tile is left out all codes have to be numbers
-            if (BITS == 8 && __builtin_amdgcn_ballot_w64(cur.pad[0] | cur.pad[1])) {
-#pragma unroll
-                for (int s = 0; s < Tile<BITS, DH>::P; ++s) {
-#pragma unroll
-                    for (int u = 0; u < Tile<BITS, DH>::NK; ++u) numbers(cur.k[u][s]);
-#pragma unroll
-                    for (int u = 0; u < Tile<BITS, DH>::NV; ++u) numbers(cur.v[u][s]);
-                }
-            }
+            // 8 bits: a code meets the other rows' zeros in the products, so a code that is no number, in a row that is left out, would reach
+            // other rows.  Seen in the result (two comparisons a tile, where cleaning all codes first cost 8 %), and done again without
+            const bool holes = BITS == 8 && __builtin_amdgcn_ballot_w64(cur.pad[0] | cur.pad[1]);
             // ---- logits of keys jt + lane and jt + 64 + lane
             float s[2];
+            for (bool again = false;; again = true) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float v = 0.f;
-                if constexpr (BITS == 4) {
+                for (int u = 0; u < 2; ++u) {
+                    float v = 0.f;
+                    if constexpr (BITS == 4) {
 #pragma unroll
-                    for (int w = NS - 1; w >= 0; --w) {
+                        for (int w = NS - 1; w >= 0; --w) {
+                            f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+                            if constexpr (DH == 32) d = mma_codes(qa[w], cur.k[u][0], d);
+                            else {
+                                d = mma_codes(qa[w], cur.k[2 * u][0], d);
+                                d = mma_codes(qb[w], cur.k[2 * u + 1][0], d);
+                            }
+                            v = fmaf(v, 0x1p-20f, join_digits(d));
+                        }
+                    } else {
                         f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-                        if constexpr (DH == 32) d = mma_codes(qa[w], cur.k[u][0], d);
-                        else {
-                            d = mma_codes(qa[w], cur.k[2 * u][0], d);
-                            d = mma_codes(qb[w], cur.k[2 * u + 1][0], d);
-                        }
-                        v = fmaf(v, 0x1p-20f, join_digits(d));
-                    }
-                } else {
-                    f32x4_t d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {             // 8 codes of every lane's 32
-                        const int p = w >> 1, e = 2 * (w & 1);
-                        if constexpr (DH == 32) d = mma_bf16(ha[w], widen8(cur.k[u][p][e], cur.k[u][p][e + 1]), d);
-                        else {
-                            d = mma_bf16(ha[w], widen8(cur.k[2 * u][p][e], cur.k[2 * u][p][e + 1]), d);
-                            d = mma_bf16(hb[w], widen8(cur.k[2 * u + 1][p][e], cur.k[2 * u + 1][p][e + 1]), d);
+                        for (int w = 0; w < 4; ++w) {             // 8 codes of every lane's 32
+                            const int p = w >> 1, e = 2 * (w & 1);
+                            if constexpr (DH == 32) d = mma_bf16(ha[w], widen8(cur.k[u][p][e], cur.k[u][p][e + 1]), d);
+                            else {
+                                d = mma_bf16(ha[w], widen8(cur.k[2 * u][p][e], cur.k[2 * u][p][e + 1]), d);
+                                d = mma_bf16(hb[w], widen8(cur.k[2 * u + 1][p][e], cur.k[2 * u + 1][p][e + 1]), d);
+                            }
                         }
-                    }
-                    v = d[0];
+                        v = d[0];
 #pragma unroll
-                    for (int i = 1; i < NQ; ++i) v += d[i];
+                        for (int i = 1; i < NQ; ++i) v += d[i];
+                    }
+                    v *= bf16_bits(cur.ks[u]) * cq;
+                    if constexpr (REL) v = fmaf(rel[hh * stretch + jt - c0 + 64 * u + lane], cs, v);
+                    s[u] = cur.pad[u] ? -INFINITY : v;
                 }
-                v *= bf16_bits(cur.ks[u]) * cq;
-                if constexpr (REL) v = fmaf(rel[hh * stretch + jt - c0 + 64 * u + lane], cs, v);
-                s[u] = cur.pad[u] ? -INFINITY : v;
+                if (!holes || again || !__builtin_amdgcn_ballot_w64(s[0] != s[0] || s[1] != s[1])) break;
+#pragma unroll
+                for (int w = 0; w < Tile<BITS, DH>::P; ++w)
+#pragma unroll
+                    for (int u = 0; u < Tile<BITS, DH>::NK; ++u) numbers(cur.k[u][w]);
             }
             // ---- running softmax
             const float mn = fmaxf(m, wave_max(fmaxf(s[0], s[1])));
@@ -742,16 +742,27 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
                 for (int w = 0; w < 4; ++w)
                     pa[w] = __builtin_bit_cast(bf16x8_t, c < NP ? *reinterpret_cast<const u32x4_t*>(pw + c * PR + 64 * g + 16 * w) : zero);
                 lds_order();
+                float v[DH / 16];
+                for (bool again = false;; again = true) {
+                    bool none = false;
 #pragma unroll
-                for (int u = 0; u < DH / 16; ++u) {
-                    f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+                    for (int u = 0; u < DH / 16; ++u) {
+                        f32x4_t d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) d = mma_bf16(pa[w], widen8(cur.v[u][w >> 1][2 * (w & 1)], cur.v[u][w >> 1][2 * (w & 1) + 1]), d);
-                    float v = d[0];
+                        for (int w = 0; w < 4; ++w) d = mma_bf16(pa[w], widen8(cur.v[u][w >> 1][2 * (w & 1)], cur.v[u][w >> 1][2 * (w & 1) + 1]), d);
+                        v[u] = d[0];
 #pragma unroll
-                    for (int i = 1; i < NP; ++i) v += d[i];
-                    acc[u] = fmaf(acc[u], alpha, v);
+                        for (int i = 1; i < NP; ++i) v[u] += d[i];
+                        none |= v[u] != v[u];
+                    }
+                    if (!holes || again || !__builtin_amdgcn_ballot_w64(none)) break;
+#pragma unroll
+                    for (int w = 0; w < Tile<BITS, DH>::P; ++w)
+#pragma unroll
+                        for (int u = 0; u < DH / 16; ++u) numbers(cur.v[u][w]);
                 }
+#pragma unroll
+                for (int u = 0; u < DH / 16; ++u) acc[u] = fmaf(acc[u], alpha, v[u]);
             }
             if (more) cur = nxt;
         }

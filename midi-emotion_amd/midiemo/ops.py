@@ -456,50 +456,52 @@ def sample_step(logits, V, special, prev_tok, is_timeshift, repeat_counts, temp_
 
 def _sample_ws(B, V, device):
     """workspace of a sampling call over wide rows: from the caching allocator, so calls on two streams or in two graphs never share one"""
-    if V <= _lib.ME_SAMPLE_ONE_BLOCK:
-        return None
     return torch.empty(lib().me_workspace_bytes(ME_WS_SAMPLE, B, V, 0, 0), dtype=torch.uint8, device=device)
 
 
-def _check_sample(logits, V, special, rows, out_ids, n_choices):
-    """B of a sampling call whose tensors fit; rows: the f32 values, one per sequence"""
-    B, dev = out_ids.numel(), logits.device
-    if not (logits.dtype is torch.float32 and logits.dim() == 2 and logits.size(0) == B and logits.size(1) >= V and logits.stride(1) == 1 and
-            out_ids.dtype is torch.int64 and out_ids.is_contiguous() and out_ids.device == dev):
-        raise RuntimeError("sampling: logits must be float32 [%d, >= %d] with contiguous rows, the picked ids contiguous int64 on their device (got %s %s, %s %s)" %
-                           (B, V, logits.dtype, tuple(logits.shape), out_ids.dtype, out_ids.device))
+def _sample_rows(B, V, logits, special, rows, ids, n_choices):
+    """The current stream and the address of each of a sampling call's tensors, all looked at first: rows = the f32 values, ids = the int64 ones, one per sequence."""
+    dev, f32 = logits.get_device(), torch.float32
+    shape, stride = logits.shape, logits.stride()
+    if not (logits.dtype is f32 and len(shape) == 2 and shape[0] == B and shape[1] >= V and stride[1] == 1):
+        raise RuntimeError("sampling: logits must be float32 [%d, >= %d] with contiguous rows (got %s %s)" % (B, V, logits.dtype, tuple(shape)))
     for x in rows:
-        if not (x.dtype is torch.float32 and x.numel() == B and x.is_contiguous() and x.device == dev):
-            raise RuntimeError("sampling: one contiguous float32 value per sequence is needed on %s (got %s %s on %s)" % (dev, x.dtype, tuple(x.shape), x.device))
+        if not (x.dtype is f32 and x.numel() == B and x.is_contiguous() and x.get_device() == dev):
+            raise RuntimeError("sampling: one contiguous float32 value per sequence is needed on %s (got %s %s on %s)" % (logits.device, x.dtype, tuple(x.shape), x.device))
+    for x in ids:
+        if not (x.dtype is torch.int64 and x.numel() == B and x.is_contiguous() and x.get_device() == dev):
+            raise RuntimeError("sampling: ids must be contiguous int64 on %s, one per sequence (got %s %s on %s)" % (logits.device, x.dtype, tuple(x.shape), x.device))
     for x, n in ((special, None), (n_choices, B)):
-        if x is not None and not (x.dtype is torch.int32 and x.is_contiguous() and x.device == dev and (n is None or x.numel() == n)):
-            raise RuntimeError("sampling: special ids and counts must be contiguous int32 on %s, counts one per sequence" % dev)
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
-        raise RuntimeError("sampling: the tensors are on %s, the current device is %d" % (dev, torch.cuda.current_device()))
-    return B
+        if x is not None and not (x.dtype is torch.int32 and x.is_contiguous() and x.get_device() == dev and (n is None or x.numel() == n)):
+            raise RuntimeError("sampling: special ids and counts must be contiguous int32 on %s, counts one per sequence" % logits.device)
+    lg = _ptr(logits)
+    if dev != torch.cuda.current_device():
+        raise RuntimeError("sampling: the tensors are on %s, the current device is %d" % (logits.device, torch.cuda.current_device()))
+    return (torch._C._cuda_getCurrentRawStream(dev), lg, stride[0], V, special.data_ptr() if special is not None else None, special.numel() if special is not None else 0,
+            [x.data_ptr() for x in rows], [x.data_ptr() for x in ids], n_choices.data_ptr() if n_choices is not None else None)
 
 
 def sample_minp(logits, V, special, temp, top_k, top_p, min_p, u, out_ids, n_choices=None):
     """one token per row of f32 logits [B, >= V] under temperature, top-k, top-p and min-p at the uniforms u (me_sample_minp)"""
-    B = _check_sample(logits, V, special, (temp, u), out_ids, n_choices)
-    ws = _sample_ws(B, V, logits.device)
-    check(lib().me_sample_minp(_ptr(logits), logits.stride(0), V, _ptr(special), special.numel() if special is not None else 0, _ptr(temp),
-                               int(top_k), float(top_p), float(min_p), _ptr(u), _ptr(out_ids), _ptr(n_choices), B, _ptr(ws), ws.numel() if ws is not None else 0, _stream()), "me_sample_minp")
+    B = out_ids.numel()
+    stream, lg, ld, V, sp, n_sp, (tm, un), (out,), nc = _sample_rows(B, V, logits, special, (temp, u), (out_ids,), n_choices)
+    ws = _sample_ws(B, V, logits.device) if V > _lib.ME_SAMPLE_ONE_BLOCK else None
+    check(lib().me_sample_minp(lg, ld, V, sp, n_sp, tm, int(top_k), float(top_p), float(min_p), un, out, nc, B, _ptr(ws), ws.numel() if ws is not None else 0,
+                               stream), "me_sample_minp")
 
 
 def sample_minp_step(logits, V, special, prev_tok, is_timeshift, repeat_counts, temp_note, temp_rest, penalty_coeff, top_k, top_p, min_p,
                      u_table, pos, pos0, out_ids, n_choices=None):
     """sample_step with min-p and for wide vocabularies (me_sample_minp_step)"""
-    B = _check_sample(logits, V, special, (repeat_counts,), out_ids, n_choices)
-    if not (prev_tok.dtype is torch.int64 and prev_tok.numel() == B and is_timeshift.dtype is torch.uint8 and is_timeshift.numel() >= V and
-            u_table.dtype is torch.float32 and u_table.dim() == 2 and u_table.size(1) >= B and u_table.stride(1) == 1 and pos.dtype is torch.int32):
-        raise RuntimeError("sampling: a step needs int64 tokens [%d], uint8 time-shift marks [>= %d], float32 uniforms [steps, >= %d] and an int32 position" % (B, V, B))
-    ws = _sample_ws(B, V, logits.device)
-    check(lib().me_sample_minp_step(_ptr(logits), logits.stride(0), V, _ptr(special), special.numel() if special is not None else 0,
-                                    _ptr(prev_tok), _ptr(is_timeshift), _ptr(repeat_counts), float(temp_note), float(temp_rest),
-                                    float(penalty_coeff), int(top_k), float(top_p), float(min_p), _ptr(u_table), u_table.stride(0), _ptr(pos),
-                                    int(pos0), _ptr(out_ids), _ptr(n_choices), B, _ptr(ws), ws.numel() if ws is not None else 0, _stream()),
-          "me_sample_minp_step")
+    B = out_ids.numel()
+    if not (is_timeshift.dtype is torch.uint8 and is_timeshift.numel() >= V and is_timeshift.is_contiguous() and u_table.dtype is torch.float32 and
+            u_table.dim() == 2 and u_table.size(1) >= B and u_table.stride(1) == 1 and pos.dtype is torch.int32):
+        raise RuntimeError("sampling: a step needs uint8 time-shift marks [>= %d], float32 uniforms [steps, >= %d] and an int32 position" % (V, B))
+    stream, lg, ld, V, sp, n_sp, (rc,), (prev, out), nc = _sample_rows(B, V, logits, special, (repeat_counts,), (prev_tok, out_ids), n_choices)
+    ws = _sample_ws(B, V, logits.device) if V > _lib.ME_SAMPLE_ONE_BLOCK else None
+    check(lib().me_sample_minp_step(lg, ld, V, sp, n_sp, prev, _ptr(is_timeshift), rc, float(temp_note), float(temp_rest), float(penalty_coeff),
+                                    int(top_k), float(top_p), float(min_p), _ptr(u_table), u_table.stride(0), _ptr(pos), int(pos0), out, nc, B,
+                                    _ptr(ws), ws.numel() if ws is not None else 0, stream), "me_sample_minp_step")
 
 
 def decode_commit(tok, history, pos, B):

@@ -229,3 +229,13 @@ def test_repeats_and_replays():
         call()
         first = ids.clone(), n.clone()
         ids.zero_()
+
+
+def test_tensors_on_the_host_are_refused():
+    from midiemo import ops
+    x, one, ids = torch.zeros(2, 50).cuda(), torch.ones(2).cuda(), torch.empty(2, dtype=torch.int64).cuda()
+    for bad in ((one.cpu(), one, ids), (one, one.cpu(), ids), (one, one, ids.cpu())):
+        with pytest.raises(RuntimeError, match="sampling: "):
+            ops.sample_minp(x, 50, None, bad[0], 0, 0.9, 0.0, bad[1], bad[2])
+    with pytest.raises(RuntimeError, match="sampling: "):
+        ops.sample_minp(x, 50, torch.zeros(1, dtype=torch.int32), one, 0, 0.9, 0.0, one, ids)
