@@ -447,7 +447,7 @@ int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
 /* ---- quantised key / value cache ------------------------------------------------------------------------------------
  * The caches of the decode step (generate.py:92-122 made incremental) in 4 or 8 bits: a row (one token, one head) of dh
  * values is held as dh codes and one bfloat16 scale,
- *   scale = amax / top, top = 6 (4 bits: e2m1) or 448 (8 bits: e4m3); f32 quotient cut (not rounded) to bfloat16,
+ *   scale = amax / top, top = 6 (4 bits: e2m1) or 448 (8 bits: e4m3); f32, amax times the rounded reciprocal, cut (not rounded) to bfloat16,
  *   code  = x / scale to the nearest value of the code's type, ties to the even code, larger ones to the largest;
  * a row with amax < 2^-96 is held as zeros (scale 0), a row with an infinity or a NaN reads back as NaN (scale NaN, codes 0).
  * 32 tokens form a block; `blocks` of them per (sequence, head) are the cache's room:

@@ -13,7 +13,7 @@ def scale_of(x, bits):
     """bfloat16-valued scales (float32) of rows x [..., dh]"""
     amax = x.float().abs().amax(-1)
     amax = torch.where(torch.isnan(x.float()).any(-1), torch.full_like(amax, math.nan), amax)
-    s = ((amax / TOP[bits]).view(torch.int32) & -65536).view(torch.float32)
+    s = ((amax * torch.tensor(1 / TOP[bits], dtype=torch.float32)).view(torch.int32) & -65536).view(torch.float32)
     s = torch.where(amax >= 2.0 ** -96, s, torch.zeros_like(s))
     return torch.where(torch.isfinite(amax), s, torch.full_like(s, math.nan))
 

@@ -49,6 +49,22 @@ def same(a, b):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+def test_scales_next_to_their_borders(bits):
+    """f32 rows whose largest value is a scale's exact multiple, or up to three bits off it"""
+    scales = torch.arange(0x3f80, 0x4080, dtype=torch.int32) << 16
+    amax = (scales.view(torch.float32) * R.TOP[bits]).view(torch.int32)[:, None] + torch.arange(-3, 4, dtype=torch.int32)
+    amax = amax.view(torch.float32).reshape(1, -1, 1, 1)                  # 1792 rows
+    x = (torch.rand(1, amax.shape[1], 1, 32, generator=torch.Generator().manual_seed(1)) - 0.5) * amax
+    x[..., 7] = amax[..., 0]
+    c = cache(1, 1, 1792, 32, bits)
+    c.write(x.cuda(), x.neg().cuda(), 0)
+    codes, scale, value = expect_rows(x, bits, torch.float32)
+    assert torch.equal(c.k_scale.cpu().float()[0, 0], scale[0, 0]) and torch.equal(c.v_scale, c.k_scale)
+    k, v = c.read(0, 1792)
+    assert same(k.cpu(), value) and same(v.cpu(), -value)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dh", [32, 48, 64])
 @pytest.mark.parametrize("T", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("n,pos,kind", [(1, 0, "plain"), (1, 37, "plain"), (1, 63, "grid"), (31, 5, "plain"), (64, 32, "grid"), (77, 45, "odd"), (200, 1, "plain")])
