@@ -5,24 +5,17 @@ A row (one token, one head) of head_dim values is held as 4-bit e2m1 or 8-bit e4
 cut to bfloat16): 34 or 66 bytes at head_dim 64 against 128 in bf16.  The codes lie in the order in which the matrix instructions take
 them (include/midiemo.h describes it), 32 tokens to a block.  The decode step this serves: generate.py:92-122 of the
 reference, made incremental; the attention is music_multi.py:211-235 for one query row."""
-import contextlib
-
 import torch
 
 from . import ops
 
 HEAD_DIMS = (32, 48, 64)
 BLOCK = 32
-_HERE = contextlib.nullcontext()
 
 
 def _need(ok, what):
     if not ok:
         raise RuntimeError("kv cache: " + what)
-
-
-def _layout(*tensors):
-    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
 
 
 class QuantKVCache:
@@ -61,8 +54,8 @@ class QuantKVCache:
         self.device = k.device
         self.nbytes = 2 * (k.numel() + 2 * k_scale.numel())
         self._index = k.device.index
-        # layouts (shapes, strides, types, devices: never addresses) that have passed the checks, with the host stride array of rows;
-        # a decode loop makes the same calls again and again, and the checks cost more host time than the launch
+        # layouts (shapes, strides, types, devices: never addresses) that have passed the checks, with what the C call takes of them; a
+        # decode loop makes the same calls again and again, and checks and arguments cost more host time than the launch
         self._seen = {}
         self.ref = ops.kvq_cache(k, k_scale, v, v_scale, head_dim, bits) if k.device.type == "cuda" else None
 
@@ -81,28 +74,34 @@ class QuantKVCache:
         return value
 
     def _pos(self, pos, n, first=0):
+        """(t, t_dev, ld_t) of a position for n rows"""
         if isinstance(pos, torch.Tensor):
             if not (pos.dtype is torch.int32 and pos.is_contiguous() and pos.numel() in (1, self.batch) and pos.device == self.device):
                 _need(False, "a position tensor must be int32 with 1 or %d values on %s" % (self.batch, self.device))
-        elif not (first <= pos and pos + n <= self.max_len):
+            return 0, pos.data_ptr(), 1 if pos.numel() > 1 else 0
+        if not (first <= pos and pos + n <= self.max_len):
             _need(False, "positions %d..%d do not fit %d tokens" % (pos, pos + n - 1, self.max_len))
+        return int(pos), None, 0
 
     def _lens(self, lens):
-        if lens is not None and not (lens.dtype is torch.int32 and lens.shape == (self.batch,) and lens.is_contiguous() and lens.device == self.device):
+        if lens is None:
+            return None
+        if not (lens.dtype is torch.int32 and lens.shape == (self.batch,) and lens.is_contiguous() and lens.device == self.device):
             _need(False, "lens must be int32 [%d] on %s" % (self.batch, self.device))
+        return lens.data_ptr()
 
     def _check_rows(self, k, v):
         for x in (k, v):
             _need(x.dim() == 4 and x.shape == k.shape and x.shape[0] == self.batch and x.shape[2:] == (self.heads, self.head_dim) and x.dtype == k.dtype and
                   (x.stride(3) == 1 or x.numel() == 0), "rows must be [%d, n, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
         _need(k.shape[1] <= self.max_len, "%d rows do not fit %d tokens" % (k.shape[1], self.max_len))
-        return ops.kvq_strides(k, v)
+        return k.shape[1], ops.kvq_strides(k, v), ops._code(k.dtype)
 
     def _check_new(self, q, k, v):
         for x in (k, v):
             _need(x.shape == (self.batch, self.heads, self.head_dim) and x.dtype == q.dtype and x.stride() == k.stride() and x.stride(2) == 1,
                   "new rows must be [%d, %d, %d] of q's type with equal strides and the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
-        return True
+        return k.stride()[:2]
 
     def _check_attend(self, q, rel, key_pad, out):
         _need(q.dim() == 3 and q.shape == (self.batch, self.heads, self.head_dim) and q.stride(2) == 1, "q must be [%d, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(q.shape)))
@@ -114,72 +113,87 @@ class QuantKVCache:
                   "key_pad must be contiguous uint8 or bool [%d, n]" % self.batch)
         if out is not None:
             _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1 and all(s != 0 or x == 1 for s, x in zip(out.stride(), out.shape)), "out must match q")
-        return True
+        o = out.stride()[:2] if out is not None else (self.heads * self.head_dim, self.head_dim)
+        return q.stride()[:2], o, rel.shape[0] if rel is not None else 0, key_pad.shape[1] if key_pad is not None else 0, ops._code(q.dtype)
 
-    def _on(self):
-        """the cache's device as the current one (nothing to do where it is)"""
+    def _elsewhere(self):
+        """the cache's device is not the current one"""
         if self.ref is None:
             _need(False, "it is on %s -- there is no CPU path" % self.device)
-        return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
+        return torch._C._cuda_getDevice() != self._index
 
     # -------------------------------------------------------------- calls
     def write(self, k, v, pos, lens=None):
         """Quantise k, v [B, n, H, head_dim] (float32, bfloat16 or float16; any strides, last dimension contiguous) into positions pos .. pos + n - 1;
         with lens (int32 [B]) only the first lens[b] rows of sequence b.  Everything else in the cache stays as it was."""
-        strides = self._passed(_layout(k, v), self._check_rows, k, v)
-        n = k.shape[1]
-        self._lens(lens)
-        self._pos(pos, n)
-        if n == 0:
-            return
-        with self._on():
-            ops.kvq_write(self.ref, k, v, pos, lens, strides)
+        self._rows("me_kvq_write", k, v, pos, lens)
 
     def read(self, pos, n, dtype=torch.float32, lens=None):
         """The rows at positions pos .. pos + n - 1 as (k, v) [B, n, H, head_dim] of `dtype`; rows from lens[b] on are zeros."""
-        _need(0 <= n <= self.max_len, "%r rows do not fit %d tokens" % (n, self.max_len))
-        self._lens(lens)
-        self._pos(pos, n)
+        if not 0 <= n <= self.max_len:
+            _need(False, "%r rows do not fit %d tokens" % (n, self.max_len))
         k = torch.empty(self.batch, n, self.heads, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        with self._on():
-            if n > 0:
-                ops.kvq_read(self.ref, k, v, pos, lens, self._passed(_layout(k, v), self._check_rows, k, v))
+        self._rows("me_kvq_read", k, v, pos, lens)
         return k, v
+
+    def _rows(self, call, k, v, pos, lens):
+        key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device)
+        n, strides, code = self._seen.get(key) or self._passed(key, self._check_rows, k, v)
+        t, t_dev, ld_t = self._pos(pos, n)
+        first = self._lens(lens)
+        if n == 0:
+            return
+        if self._elsewhere():
+            with torch.cuda.device(self._index):
+                return self._rows(call, k, v, pos, lens)
+        ops.check(getattr(ops.lib(), call)(self.ref, k.data_ptr(), v.data_ptr(), strides, n, t, t_dev, ld_t, first, code,
+                                           torch._C._cuda_getCurrentRawStream(self._index)), call)
 
     def append_attend(self, q, k, v, pos, rel=None, key_pad=None, out=None, nsplit=0):
         """A decode step in one launch: write the rows k, v [B, H, head_dim] at pos, then attend to the keys 0 .. pos.  k and v are of q's type with
         equal strides, their rows 16-byte aligned."""
-        self._passed(_layout(q, k, v, None), self._check_new, q, k, v)
+        key = (q.dtype, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device)
+        strides = self._seen.get(key) or self._passed(key, self._check_new, q, k, v)
         self._pos(pos, 1)
-        return self.attend(q, pos, rel, key_pad, out, nsplit, (k, v))
+        return self.attend(q, pos, rel, key_pad, out, nsplit, (k, v, strides))
 
-    def attend(self, q, pos, rel=None, key_pad=None, out=None, nsplit=0, _rows=None):
+    def attend(self, q, pos, rel=None, key_pad=None, out=None, nsplit=0, _new=None):
         """softmax((q.k_j + q.rel[M-1-(pos-j)]) / sqrt(head_dim)) v over the cached keys j = 0 .. pos (pos = -1: none).
 
         q [B, H, head_dim]; rel [M, head_dim] of q's type with M >= max_len (the model's relative table) or None; key_pad uint8 / bool
         [B, n], 1 = masked key.  A row without a key gives zeros.  nsplit: key ranges that run side by side (0: chosen from the sizes)."""
         if key_pad is not None and key_pad.dtype is torch.bool:
             key_pad = key_pad.view(torch.uint8)
-        self._passed(_layout(q, rel, key_pad, out, None), self._check_attend, q, rel, key_pad, out)
-        self._pos(pos, 1 if isinstance(pos, torch.Tensor) or pos >= 0 else 0, -1)
+        key = (q.shape, q.stride(), q.dtype, q.device, rel is not None and (rel.shape, rel.stride(), rel.dtype, rel.device),
+               key_pad is not None and (key_pad.shape, key_pad.stride(), key_pad.dtype, key_pad.device), out is not None and (out.shape, out.stride(), out.dtype, out.device))
+        (qb, qh), (ob, oh), M, width, code = self._seen.get(key) or self._passed(key, self._check_attend, q, rel, key_pad, out)
+        t, t_dev, ld_t = self._pos(pos, 1 if isinstance(pos, torch.Tensor) or pos >= 0 else 0, -1)
         tokens = self.max_len
-        if not isinstance(pos, torch.Tensor):
-            tokens = max(pos + 1, 1)
-            if key_pad is not None and key_pad.shape[1] <= pos:
-                _need(False, "key_pad is narrower than the %d keys" % (pos + 1))
+        if t_dev is None:
+            tokens = max(t + 1, 1)
+            if key_pad is not None and width <= t:
+                _need(False, "key_pad is narrower than the %d keys" % (t + 1))
         if not 0 <= nsplit <= 64:
             _need(False, "nsplit must be 0..64")
-        with self._on():
-            if out is None:
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            ns = nsplit or self._splits(tokens, rel is not None)
+        if self._elsewhere():
+            with torch.cuda.device(self._index):
+                return self.attend(q, pos, rel, key_pad, out, nsplit, _new)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ns = nsplit or self._splits(tokens, rel is not None)
+        size, part = 0, None
+        if ns > 1:
             # the records of this call: from the caching allocator, so calls on two streams or in two captured graphs never share them
-            part = torch.empty(self.batch * self.heads * ns * (self.head_dim + 4), dtype=torch.float32, device=self.device) if ns > 1 else None
-            if _rows:
-                ops.kvq_append_attn(self.ref, q, _rows[0], _rows[1], out, pos, rel, key_pad, part, ns)
-            else:
-                ops.kvq_attn(self.ref, q, out, pos, rel, key_pad, part, ns)
+            size = self.batch * self.heads * ns * (self.head_dim + 4) * 4
+            part = torch.empty(size, dtype=torch.uint8, device=self.device)
+        tail = (rel.data_ptr() if M else None, M, key_pad.data_ptr() if key_pad is not None else None, width, out.data_ptr(), ob, oh,
+                part.data_ptr() if size else None, size, ns, t, t_dev, ld_t, code, torch._C._cuda_getCurrentRawStream(self._index))
+        if _new is None:
+            ops.check(ops.lib().me_kvq_attn(self.ref, q.data_ptr(), qb, qh, *tail), "me_kvq_attn")
+        else:
+            k, v, (nb, nh) = _new
+            ops.check(ops.lib().me_kvq_append_attn(self.ref, q.data_ptr(), qb, qh, k.data_ptr(), v.data_ptr(), nb, nh, *tail), "me_kvq_append_attn")
         return out
 
     def _splits(self, tokens, rel):
