@@ -175,12 +175,25 @@ template <int NT> struct __attribute__((aligned(16))) Shared {
     uint32_t r32[NT / 64], found_bin, found_rank, n_list;
 };
 
+// inclusive sums over a wave's lanes by lane moves of the vector unit (six steps; through LDS each step is a round trip)
+template <int CTRL, int ROWS> ME_DEV uint32_t moved(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS> ME_DEV u64 moved(u64 x) { return ((u64)moved<CTRL, ROWS>((uint32_t)(x >> 32)) << 32) | moved<CTRL, ROWS>((uint32_t)x); }
+template <typename T> ME_DEV T wave_scan(T x) {
+    x += moved<0x111, 0xF>(x);                                // 1, 2, 4, 8 lanes on inside the rows of 16
+    x += moved<0x112, 0xF>(x);
+    x += moved<0x114, 0xF>(x);
+    x += moved<0x118, 0xF>(x);
+    x += moved<0x142, 0xA>(x);                                // a row's last lane to the next row (rows 1 and 3)
+    x += moved<0x143, 0xC>(x);                                // lane 31 to rows 2 and 3
+    return x;
+}
 // three sums at once
 template <int NT> ME_DEV void block_sum3(Shared<NT>& s, uint32_t& n, u64& x, u64& y) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) { n += __shfl_xor(n, o); x += __shfl_xor(x, o); y += __shfl_xor(y, o); }
+    n = wave_scan(n);
+    x = wave_scan(x);
+    y = wave_scan(y);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) { s.r32[threadIdx.x >> 6] = n; s.r64[threadIdx.x >> 6] = x; s.q64[threadIdx.x >> 6] = y; }
+    if ((threadIdx.x & 63) == 63) { s.r32[threadIdx.x >> 6] = n; s.r64[threadIdx.x >> 6] = x; s.q64[threadIdx.x >> 6] = y; }
     __syncthreads();
     n = 0; x = 0; y = 0;
 #pragma unroll
@@ -215,14 +228,8 @@ template <int NT, int N> ME_DEV void scan_bins(Shared<NT>& s, uint32_t* cnt, u64
     u64 m[PB], ms = 0;
 #pragma unroll
     for (int i = 0; i < PB; ++i) { c[i] = on ? cnt[tid * PB + i] : 0; m[i] = on ? mass[tid * PB + i] : 0; cs += c[i]; ms += m[i]; }
-    uint32_t ci = cs;
-    u64 mi = ms;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(ci, o);
-        const u64 y = __shfl_up(mi, o);
-        if (lane >= o) { ci += x; mi += y; }
-    }
+    const uint32_t ci = wave_scan(cs);
+    const u64 mi = wave_scan(ms);
     __syncthreads();
     if (lane == 63) { s.r32[wid] = ci; s.r64[wid] = mi; }
     __syncthreads();
@@ -252,9 +259,7 @@ template <int NT> ME_DEV void scan_mass(Shared<NT>& s, u64* mass, u64& m_all) {
     u64 m[PB], ms = 0;
 #pragma unroll
     for (int i = 0; i < PB; ++i) { m[i] = mass[tid * PB + i]; ms += m[i]; }
-    u64 mi = ms;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(mi, o); if (lane >= o) mi += y; }
+    const u64 mi = wave_scan(ms);
     __syncthreads();
     if (lane == 63) s.r64[wid] = mi;
     __syncthreads();
