@@ -322,22 +322,41 @@ template <int NT> ME_DEV Barred bar_ids(const SampleArgs& a, uint32_t* bits, int
     __syncthreads();
     return {bits + 1, j0 + (int)__builtin_amdgcn_readfirstlane((int)bits[0])};
 }
-// entries [j0, j1) of a row, once each: NaN -> 0, barred ids -> -inf; f(value, index)
+// entries [j0, j1) of a row, once each: NaN -> 0, barred ids -> -inf; f(value, index).  Whole blocks of NT * U behind the barred ids, nearly all
+// of a row, are read without a bound and without the look at the bits: about a third of a walk's instructions
 template <int NT, int U, typename F> ME_DEV void each_entry(const float* lg, int j0, int j1, const Barred& barred, F&& f) {
-    for (int i0 = j0 + (int)threadIdx.x; i0 < j1; i0 += NT * U) {
-        float x[U];
+    const int tid = threadIdx.x;
+    int b0 = j0;                                              // uniform
+#pragma clang loop unroll(disable)
+    for (int part = 0; part < 2; ++part) {
+        const int stop = part ? j1 : min(j1, j0 + (max(barred.end, j0) - j0 + NT * U - 1) / (NT * U) * (NT * U));
+        for (; b0 < stop; b0 += NT * U) {
+            float x[U];
 #pragma unroll
-        for (int q = 0; q < U; ++q) x[q] = lg[min(i0 + q * NT, j1 - 1)];
+            for (int q = 0; q < U; ++q) x[q] = lg[min(b0 + q * NT + tid, j1 - 1)];
 #pragma unroll
-        for (int q = 0; q < U; ++q) {
-            const int j = i0 + q * NT;
-            if (j < j1) {
-                float v = x[q];
-                if (v != v) v = 0.f;
-                if (j < barred.end && ((barred.bits[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u)) v = -INFINITY;
-                f(v, j);
+            for (int q = 0; q < U; ++q) {
+                const int j = b0 + q * NT + tid;
+                if (j < j1) {
+                    float v = x[q];
+                    if (v != v) v = 0.f;
+                    if (j < barred.end && ((barred.bits[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u)) v = -INFINITY;
+                    f(v, j);
+                }
+                __builtin_amdgcn_sched_barrier(0);            // the entries' f64 chains stay apart (the waves hide them): few registers
             }
-            __builtin_amdgcn_sched_barrier(0);                // the entries' f64 chains stay apart (the waves hide them): few registers
+        }
+        if (part) break;
+        for (; b0 + NT * U <= j1; b0 += NT * U) {
+            const float* p = lg + b0;
+            float x[U];
+#pragma unroll
+            for (int q = 0; q < U; ++q) x[q] = p[q * NT + tid];
+#pragma unroll
+            for (int q = 0; q < U; ++q) {
+                f(x[q] != x[q] ? 0.f : x[q], b0 + q * NT + tid);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
 }
@@ -748,12 +767,11 @@ __global__ __launch_bounds__(WT) void sample_gather_kernel(const SampleArgs a) {
     float v_lo[3], v_hi[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) sc.interval(lo[i], hi[i], v_lo[i], v_hi[i]);
-    each_entry<WT, 8>(a.logits + (size_t)b * a.ld, j0, j1, barred, [&](float v, int j) {
-        if ((v >= v_lo[0] && v <= v_hi[0]) || (v >= v_lo[1] && v <= v_hi[1]) || (v >= v_lo[2] && v <= v_hi[2])) {
-            const uint32_t k = atomicAdd(&s.n_list, 1u);
-            if (k < (uint32_t)SL) mine[k] = word_of(v, j);
-        }
-    });
+    auto keep = [&](float v, int j) { const uint32_t k = atomicAdd(&s.n_list, 1u); if (k < (uint32_t)SL) mine[k] = word_of(v, j); };
+    auto in = [&](float v, int i) { return v >= v_lo[i] && v <= v_hi[i]; };
+    const float* lg = a.logits + (size_t)b * a.ld;
+    if (cuts(a)) each_entry<WT, 8>(lg, j0, j1, barred, [&](float v, int j) { if (in(v, 0) || in(v, 1) || in(v, 2)) keep(v, j); });
+    else each_entry<WT, 8>(lg, j0, j1, barred, [&](float v, int j) { if (in(v, 1) || in(v, 2)) keep(v, j); });
     __syncthreads();
     const uint32_t n = s.n_list;
     if (tid == 0) base = n ? atomicAdd(w.n_list, n > (uint32_t)SL ? (uint32_t)GL + 1 : n) : 0;      // at most MAX_SPLIT of these: no overflow
