@@ -15,10 +15,10 @@
 // row, bins and lists in its LDS.  Wider ones take four launches: the chunks' maxima; the chunks' histograms; the members of
 // the bins that can hold one of the borders (known up to a bin or two from the histogram alone), gathered by all chunks; and one block per
 // row that finishes on those few entries.  Measured, us a call in a graph, top_p 0.9 and min_p 0.05 / top_k 200, top_p 0.95 and min_p 0.02:
-//   one block, 256 threads:   4 x 1018: 10.0 / 13.5,  64 x 2048: 11.2 / 15.3,  512 x 1018: 11.2 / 15.3
-//   one block, 1024 threads:  64 x 32000: 26.5 / 26.1 (0.31 TB/s: 64 of 256 CUs),  256 x 32512: 29.7 / 30.5 (1.1 TB/s)
-//   four launches:            1 x 131071: 31.7 / 39.5,  128 x 131071: 74.7 / 84.0 (0.9 TB/s; the row is read three times, from the
-//                             last-level cache: maxima 12, histograms 31, gathering 27, finish 16 us)
+//   one block, 256 threads:   4 x 1018: 7.6 / 12.7,  64 x 2048: 10.5 / 14.5,  512 x 1018: 10.4 / 14.1
+//   one block, 1024 threads:  64 x 32000: 23.7 / 24.2 (0.34 TB/s: 64 of 256 CUs),  256 x 32512: 29.6 / 28.3 (1.2 TB/s)
+//   four launches:            1 x 131071: 27.7 / 32.4,  128 x 131071: 64.7 / 76.9 (1.0 TB/s; the row is read three times, from the
+//                             last-level cache: maxima 12, histograms 28, gathering 20, finish 15 us)
 #include "me_common.h"
 #include <algorithm>
 #include <math.h>
@@ -35,7 +35,7 @@ constexpr int NL = 128;                     // entries that are compared with ea
 constexpr int GL = 4096;                    // gathered entries of a wide row
 constexpr int FRAC = 45;                    // weight unit 2^-45
 // 32512: the row, the bins and the lists fill 160 KB of LDS.  Up to there one block is faster at every batch measured, although
-// few rows leave CUs idle: 32512 symbols in one block / 32513 in four launches, us: 1 row 23.8 / 26.2, 8: 24.4 / 28.8, 64: 25.1 / 39.2, 512: 57.2 / 75.8
+// few rows leave CUs idle: 32512 symbols in one block / 32513 in four launches, us: 1 row 22.3 / 25.3, 8: 22.8 / 28.4, 64: 23.4 / 38.6, 512: 53.2 / 66.1
 constexpr int ONE_BLOCK = ME_SAMPLE_ONE_BLOCK;
 constexpr int MAX_SPLIT = 16;               // chunks of a wide row at most: every later block reads all chunks' histograms
 
@@ -510,7 +510,7 @@ ME_DEV void choose(const SampleArgs& a, int b, float u, uint32_t n_keep, u64 m_k
 // ---------------------------------------------------------------------------------------------------------
 // rows of up to ONE_BLOCK symbols: one block, the row in LDS.  Without top-k one walk makes the histogram of what min-p keeps.  With
 // top-k the walk only counts, and the few entries up to its border's bin are collected; they alone get weights and take the row's place
-// in the searches (64 x 32000, top_k 200: 26 us; 32 when the row was walked again for each search).
+// in the searches (64 x 32000, top_k 200: 24 us; 32 when the row was walked again for each search).
 // ---------------------------------------------------------------------------------------------------------
 template <int NT>
 __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
@@ -620,8 +620,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// wider rows: grid (splits, B) blocks of a chunk each.  Bounded by the histogram's and the gathering's instructions, about 40 an entry
-// (128 x 131071: 31 and 27 us; their bytes alone would take 13 us each at the rate of a copy)
+// wider rows: grid (splits, B) blocks of a chunk each.  Bounded by the histogram's and the gathering's instructions, about 30 an entry
+// (128 x 131071: 28 and 20 us; their bytes alone would take 13 us each at the rate of a copy)
 // ---------------------------------------------------------------------------------------------------------
 constexpr int WT = 512;                                       // threads of a chunk's block
 constexpr int PT = 256;                                       // and of the block that finishes a row
@@ -841,7 +841,7 @@ int splits_of(int B, int V) { return std::max(1, std::min(std::min(512 / std::ma
 int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st) {
     static bool big1[64] = {}, big2[64] = {};
     if (a.V <= ONE_BLOCK) {
-        // 256 threads to 2048 symbols: fewer waves meet at each barrier (2048 symbols on 256 / 2049 on 1024 threads: 4 rows 10.9 / 12.0 us, 64: 11.2 / 14.1)
+        // 256 threads to 2048 symbols: fewer waves meet at each barrier (2048 symbols on 256 / 2049 on 1024 threads: 4 rows 8.4 / 10.5 us, 64: 10.5 / 12.7)
         if (a.V <= 2048) sample_row_kernel<256><<<B, 256, sizeof(Shared<256>) + SL * 8 + (size_t)(a.V + 3) / 4 * 16, st>>>(a);
         else {
             static_assert(sizeof(Shared<1024>) + SL * 8 + (size_t)ONE_BLOCK * 4 <= 160 * 1024, "the widest row of one block");
