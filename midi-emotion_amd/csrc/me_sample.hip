@@ -36,6 +36,7 @@ constexpr int GL = 4096;                    // gathered entries of a wide row
 constexpr int FRAC = 45;                    // weight unit 2^-45
 // 32512: the row, the bins and the lists fill 160 KB of LDS.  Up to there one block is faster at every batch measured, although
 // few rows leave CUs idle: 32512 symbols in one block / 32513 in four launches, us: 1 row 22.3 / 25.3, 8: 22.8 / 28.4, 64: 23.4 / 38.6, 512: 53.2 / 66.1
+// (top_p 0.9, min_p 0.05; where a border falls into a full bin both take longer, and for a single row it was 31.3 / 25.9)
 constexpr int ONE_BLOCK = ME_SAMPLE_ONE_BLOCK;
 constexpr int MAX_SPLIT = 16;               // chunks of a wide row at most: every later block reads all chunks' histograms
 
@@ -199,16 +200,25 @@ template <int NT> ME_DEV void block_sum3(Shared<NT>& s, uint32_t& n, u64& x, u64
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) { n += s.r32[w]; x += s.r64[w]; y += s.q64[w]; }
 }
-template <int NT> ME_DEV u64 block_max64(Shared<NT>& s, u64 v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) { const u64 x = __shfl_xor(v, o); v = x > v ? x : v; }
+ME_DEV u64 larger(u64 a, u64 b) { return a > b ? a : b; }
+ME_DEV u64 wave_top(u64 x) {                                  // in lane 63
+    x = larger(x, moved<0x111, 0xF>(x));
+    x = larger(x, moved<0x112, 0xF>(x));
+    x = larger(x, moved<0x114, 0xF>(x));
+    x = larger(x, moved<0x118, 0xF>(x));
+    x = larger(x, moved<0x142, 0xA>(x));
+    return larger(x, moved<0x143, 0xC>(x));
+}
+// two maxima at once
+template <int NT> ME_DEV void block_max64(Shared<NT>& s, u64& x, u64& y) {
+    x = wave_top(x);
+    y = wave_top(y);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.r64[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) { s.r64[threadIdx.x >> 6] = x; s.q64[threadIdx.x >> 6] = y; }
     __syncthreads();
-    u64 t = 0;
+    x = 0; y = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) t = s.r64[w] > t ? s.r64[w] : t;
-    return t;
+    for (int w = 0; w < NT / 64; ++w) { x = larger(s.r64[w], x); y = larger(s.q64[w], y); }
 }
 template <int NT> ME_DEV float block_max(Shared<NT>& s, float v) {
     v = wave_max(v);
@@ -453,8 +463,8 @@ ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, double y_floor, 
         u64 wmax = 0, wmin = 0;                               // wmin as the maximum of the complement
         window([&](u64 w) { wmax = max(wmax, w); wmin = max(wmin, ~w); });
         for (int i = tid; i < NB1; i += NT) { s.cnt1[i] = 0; s.mass1[i] = 0; }
-        wmax = block_max64(s, wmax);
-        wmin = ~block_max64(s, wmin);
+        block_max64(s, wmax, wmin);
+        wmin = ~wmin;
         const int width = 64 - (int)__builtin_clzll((wmax - wmin) | 1);
         const int next = max(0, width - 8);                   // 2^8 = NB1 pieces
         window([&](u64 w) {
