@@ -404,7 +404,11 @@ ME_DEV void search(Shared<NT>& s, const Scale& sc, EACH&& each, double y_floor, 
         const uint32_t cb = c0 + cnt[bin], n = c0 + (bin + 1 < nb ? cnt[bin + 1] : total) - cb;
         const u64 mb = m0 + mass[bin];
         if (level == 0) bin0 = bin;
-        else { const u64 top = hi - ((u64)bin << shift); lo = max(lo, top - (((u64)1 << shift) - 1)); hi = top; }
+        else {                                                // the piece's words; its lower end may lie below zero (words are as small as 2^55)
+            const u64 top = hi - ((u64)bin << shift), span = ((u64)1 << shift) - 1;
+            lo = max(lo, top > span ? top - span : 0);
+            hi = top;
+        }
         c0 = cb;
         m0 = mb;
         if (level == 0) sc.interval(bin0, bin0, v_lo, v_hi);

@@ -1,0 +1,30 @@
+"""me_sample_minp where a search's border lies among the entries that cannot be picked, and at the ends of the number range: against the
+same 64-bit rules as test_sample_minp_gpu.py."""
+import math
+
+import pytest
+import torch
+
+from test_sample_minp_gpu import compare
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("V", [3000, 8192, 32000, 40000])
+@pytest.mark.parametrize("masked", [-math.inf, torch.finfo(torch.float32).min])
+def test_top_k_ends_among_masked_entries(V, masked):
+    """more of top_k than there are entries to pick from: the last bin (32 temperatures below the maximum) holds positive logits next to masked ones,
+    so its entries' images span the whole 64-bit range"""
+    g = torch.Generator().manual_seed(V)
+    temp = torch.tensor([0.1, 0.2, 0.3, 0.1, 0.2, 0.3, 0.15])
+    last = torch.tensor([1.5, 1.5, 1.5, 6.0, 6.0, 6.0, 24.0])     # where the last bin begins, about
+    x = torch.randn(len(temp), V, generator=g) * 2.5
+    x = torch.minimum(x, torch.tensor(8.0))
+    x += (last + 32 * temp - x.amax(1))[:, None]
+    n = max(300, V // 30)
+    for b in range(len(temp)):
+        x[b, torch.randperm(V, generator=g)[:n]] = masked
+    special = [0, 1, 2]
+    for top_k in (V - n + 1, V - 1, V - len(special) + 1, V - n // 2):
+        for top_p, min_p in ((0.7, 0.0), (0.98, 0.0), (1.0, 0.0), (0.9, 0.05)):
+            compare(x, special, temp, top_k, top_p, min_p, torch.rand(len(temp), generator=g))
