@@ -118,7 +118,8 @@ struct Scale {
     // an interval of values that holds bins lo .. hi, a little wider: bins fall with the value, and two comparisons cost a fifth of a bin
     ME_DEV void interval(int lo, int hi, float& v_lo, float& v_hi) const {
         const bool any = lo <= hi;
-        const float slack = 1e-5f * fabsf(mx), at = (float)lo / bin_c, to = (float)(hi + 1) / bin_c;
+        const float slack = 1e-5f * fabsf(mx), to = (float)(hi + 1) / bin_c;
+        const float at = fminf((float)lo / bin_c, 3.402823466e38f);       // differences past 32 bits are in the last bin: it begins no later than there
         v_hi = !any ? -INFINITY : lo == 0 ? INFINITY : inf ? 3.402823466e38f : mx - at * 0.9999f + slack;
         v_lo = !any || (inf && hi < NB - 1) ? INFINITY : hi >= NB - 1 ? -INFINITY : mx - to * 1.0001f - slack;
     }

@@ -28,3 +28,17 @@ def test_top_k_ends_among_masked_entries(V, masked):
     for top_k in (V - n + 1, V - 1, V - len(special) + 1, V - n // 2):
         for top_p, min_p in ((0.7, 0.0), (0.98, 0.0), (1.0, 0.0), (0.9, 0.05)):
             compare(x, special, temp, top_k, top_p, min_p, torch.rand(len(temp), generator=g))
+
+
+@pytest.mark.parametrize("V", [40, 5000, 40000])
+def test_logits_of_the_whole_range_at_the_largest_temperatures(V):
+    """a bin's upper border in logits, lo / 32 times the temperature, does not fit 32 bits; differences of logits do not either"""
+    x = torch.linspace(-3e38, 3e38, V, dtype=torch.float64).float().flip(0).repeat(4, 1)
+    x[1] = x[1].roll(V // 3)
+    x[2, V // 2:] = torch.finfo(torch.float32).min
+    x[3, ::3] = -math.inf
+    top = torch.finfo(torch.float32).max
+    u = torch.tensor([0.99, 0.7, 0.9999, 0.5])
+    for temp in (torch.tensor([top, 3e38, 1e38, top]), torch.full((4,), 2e37)):
+        for top_k, top_p, min_p in ((0, 1.0, 0.0), (V - V // 8, 1.0, 0.0), (V - 1, 0.98, 0.1), (0, 0.9, 0.0)):
+            compare(x, [], temp, top_k, top_p, min_p, u)
