@@ -533,7 +533,7 @@ int me_sample_step(const float* logits, int ld, int V, const int32_t* special, i
  * out_ids[b] = the first kept entry at which the cumulative weight exceeds u[b] times the sum of the kept ones (u in [0, 1); a u of 1 and
  * more: the last one that has a weight); n_choices[b] (may be NULL) = number of kept entries.  A row with every logit -inf: id 0, 0 choices;
  * several +inf share the weight.  Cumulative weights are exact sums of weights rounded to 2^-45, so results do not depend on scheduling.
- * A temperature that is not positive (or NaN) counts as 0: the largest entries alone have a weight.  ws: me_workspace_bytes(ME_WS_SAMPLE, B, V, 0, 0) bytes, 16-byte aligned, uninitialised, private to the call
+ * A temperature that is not positive (or NaN) counts as 0: the largest entries alone have a weight; an infinite one counts as the largest f32.  ws: me_workspace_bytes(ME_WS_SAMPLE, B, V, 0, 0) bytes, 16-byte aligned, uninitialised, private to the call
  * until it has run (NULL where that is 0).
  * me_sample_minp_step is the same for a step of a device-resident loop (arguments of me_sample_step). */
 #define ME_SAMPLE_MAX_VOCAB (1 << 18)

@@ -45,7 +45,7 @@ struct SampleArgs {
     const int32_t* special; int n_special;
     const float* temp;
     int top_k; float top_p;
-    double y_min;                           // log2(min_p)
+    double y_min;                           // least_exponent(min_p)
     const float* u;
     int64_t* out; int32_t* choices;
     // a step of a device-resident loop (prev != NULL): temperature from the token just fed, uniform from a table, repeat counter
@@ -853,6 +853,9 @@ template <typename K> bool allow_lds(K kernel, size_t bytes, size_t fixed, bool 
 // chunks of a wide row: two blocks for each CU over the batch, 2048 symbols a chunk at least
 int splits_of(int B, int V) { return std::max(1, std::min(std::min(512 / std::max(B, 1), (V + 2047) / 2048), MAX_SPLIT)); }
 
+// the least exponent whose weight, rounded to 64 bits, reaches min_p: half a step of the 64 bits below 1 (all that are 1 in 64 bits pass a min_p of 1)
+double least_exponent(float min_p) { return log2((double)min_p) - 0x1p-54 * 1.4426950408889634074; }
+
 int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st) {
     static bool big1[64] = {}, big2[64] = {};
     if (a.V <= ONE_BLOCK) {
@@ -896,7 +899,7 @@ int me_sample_minp(const float* logits, int ld, int V, const int32_t* special, i
     if (B == 0) return ME_OK;
     SampleArgs a = {};
     a.logits = logits; a.ld = ld; a.V = V; a.special = special; a.n_special = n_special; a.temp = temp; a.top_k = top_k; a.top_p = top_p;
-    a.y_min = log2((double)min_p); a.u = u; a.out = out_ids; a.choices = n_choices;
+    a.y_min = least_exponent(min_p); a.u = u; a.out = out_ids; a.choices = n_choices;
     return sample_call(a, B, ws, ws_bytes, (hipStream_t)stream);
 }
 
@@ -910,7 +913,7 @@ int me_sample_minp_step(const float* logits, int ld, int V, const int32_t* speci
     if (B == 0) return ME_OK;
     SampleArgs a = {};
     a.logits = logits; a.ld = ld; a.V = V; a.special = special; a.n_special = n_special; a.top_k = top_k; a.top_p = top_p;
-    a.y_min = log2((double)min_p); a.u = u_table; a.out = out_ids; a.choices = n_choices;
+    a.y_min = least_exponent(min_p); a.u = u_table; a.out = out_ids; a.choices = n_choices;
     a.prev = prev_tok; a.is_timeshift = is_timeshift; a.repeats = repeat_counts; a.pos = pos; a.pos0 = pos0; a.u_ld = u_ld;
     a.temp_note = temp_note; a.temp_rest = temp_rest; a.penalty = penalty_coeff;
     return sample_call(a, B, ws, ws_bytes, (hipStream_t)stream);

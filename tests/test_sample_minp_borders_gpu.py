@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_sample_minp_gpu import compare
+from test_sample_minp_gpu import compare, reference, sample
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,20 @@ def test_logits_of_the_whole_range_at_the_largest_temperatures(V):
     for temp in (torch.tensor([top, 3e38, 1e38, top]), torch.full((4,), 2e37)):
         for top_k, top_p, min_p in ((0, 1.0, 0.0), (V - V // 8, 1.0, 0.0), (V - 1, 0.98, 0.1), (0, 0.9, 0.0)):
             compare(x, [], temp, top_k, top_p, min_p, u)
+
+
+@pytest.mark.parametrize("V", [40, 5000, 40000])
+def test_weights_that_are_one_in_64_bits_pass_a_min_p_of_one(V):
+    """logits that differ by less than 2^-54 temperatures: exp() of 64 bits is 1, and 1 >= 1 keeps them all"""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(4, V, generator=g)
+    x[0] *= 1e-38
+    x[1] *= 1e-20
+    x[2, V // 2] = -math.inf
+    temp = torch.tensor([1.0, 0.5, math.inf, 1e30])
+    u = torch.tensor([0.1, 0.4, 0.6, 0.9])
+    for top_k, top_p in ((0, 1.0), (V // 2, 1.0), (0, 0.9), (V - 1, 0.5)):
+        ids, n = sample(x, [], temp, top_k, top_p, 1.0, u)
+        for b in range(4):                                       # an infinite temperature counts as the largest number (-inf / inf is none)
+            want, (lo, hi) = reference(x[b].numpy(), [], temp[b].clamp(max=torch.finfo(torch.float32).max), top_k, top_p, 1.0, u[b])
+            assert ids[b] in want and lo <= n[b] <= hi, (b, ids[b], want, n[b], (lo, hi))
