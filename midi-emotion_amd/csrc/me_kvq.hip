@@ -9,7 +9,7 @@
 // of all sizes it lost up to 2^-11 of the largest product (measured).  Digit times code is a multiple of 1/2 below 97, so
 // its sums are exact.  Four digits leave 2^-19 of the largest value, six (f32) 2^-29.
 // 8 bits: e4m3 codes span 2^17, so they are widened to bfloat16 (exactly, two per instruction) for the bf16 product, which adds in
-// 32 bits; the query and the weights enter as one to three bfloat16 parts, again in the idle rows.
+// 32 bits; the query (scaled by a power of two too) and the weights enter as one to three bfloat16 parts, again in the idle rows.
 //
 // Layout of a block of 32 tokens (one head), in the order of the operands; a code's position counts codes:
 //   K: the contraction runs over dh, so 32 of a row's codes form a lane's chunk.  4 bits: chunk (group, lane) at (group * 16 + lane) * 32
@@ -494,11 +494,11 @@ __global__ __launch_bounds__(64 * WAVES) void kvq_attn_kernel(const AttnArgs a) 
     {
         float x = lane < DH ? qs[hh][lane] : 0.f;
         if (__builtin_amdgcn_ballot_w64(!(fabsf(x) <= 3.402823466e38f))) { qinv = __builtin_nanf(""); x = 0.f; }   // an infinity or a NaN in the query: every logit is NaN
+        float f, fi;                                          // 8 bits: products with codes up to 448 stay inside f32 whatever the query's size
+        unit(wave_max(fabsf(x)), f, fi);
+        qinv *= fi;
+        x *= f;
         if constexpr (BITS == 4) {
-            float f, fi;
-            unit(wave_max(fabsf(x)), f, fi);
-            qinv *= fi;
-            x *= f;
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 const float d = rintf(x);
