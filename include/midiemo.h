@@ -459,8 +459,8 @@ int me_dec_token_blocks(int dh, int d, int d_inner, int dtype);
  *   V, 4 bits: p = d * 32 + token
  *   8 bits: K: p = (i / 16) * 16 dh + (group * 16 + token % 16) * 16 + i % 16;  V: p = (token / 16) * 16 dh + d * 16 + token % 16
  * dh in {32, 48, 64}.  Positions: t for all sequences, or t_dev (device int32, may be NULL) = one value for all (ld_t = 0) or one
- * per sequence (ld_t = 1); a device position is read by the kernels and never checked by the host: tokens that have no place in the
- * cache are left out.
+ * per sequence (ld_t = 1); a device position is read by the kernels and never checked by the host: rows past the cache's end are left
+ * out, and so is a whole sequence whose position is negative or past the end (nothing written, read as zeros).
  *
  * me_kvq_write: rows [B][n][H][dh] of T (strides: six element counts {k: sequence, token, head, v: sequence, token, head}, dh
  *   contiguous; a HOST array read during the call) to positions t .. t + n - 1.  lens (device int32 [B] or NULL): only the first

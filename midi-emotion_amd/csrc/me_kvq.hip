@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void kvq_write_kernel(const RowArgs a) {
     __shared__ uint32_t vq[KB][8 * W];
     const int tid = threadIdx.x, key = tid >> 3, sub = tid & 7, h = blockIdx.y, b = blockIdx.z;
     const int t = pos_of(a.t, a.t_dev, a.ld_t, b);
-    if (t < 0 || t >= a.blocks * KB) return;                  // block-uniform: nothing of this sequence has a place
+    if (t < 0 || t >= a.blocks * KB) return;                  // block-uniform: a sequence that does not begin in the cache is left out
     const int nb = a.lens ? min(a.n, a.lens[b]) : a.n;
     const int end = (int)min((int64_t)t + nb, (int64_t)a.blocks * KB);
     const int blk = t / KB + blockIdx.x, j0 = blk * KB;

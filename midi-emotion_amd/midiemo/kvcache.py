@@ -22,8 +22,9 @@ class QuantKVCache:
     """Cache of `batch` sequences, `heads` heads, at least `max_len` tokens (rounded up to blocks of 32).
 
     Positions (`pos` below) are a whole number, or an int32 device tensor of one value or one per sequence; those are read on the
-    device (so a captured step can advance them) and rows without a place in the cache are then left out instead of
-    refused.  Calls only enqueue work on the current stream of the cache's device."""
+    device (so a captured step can advance them), and what has no place is then left out instead of refused: rows past the cache's end,
+    and a whole sequence whose position is negative or past the end.  Calls only enqueue work on the current stream of the
+    cache's device.  None of them is differentiable: results carry no gradient."""
 
     def __init__(self, batch, heads, max_len, head_dim, bits=4, device="cuda"):
         _need(batch > 0 and heads > 0 and max_len > 0, "batch, heads and max_len must be positive")
@@ -162,7 +163,7 @@ class QuantKVCache:
         """softmax((q.k_j + q.rel[M-1-(pos-j)]) / sqrt(head_dim)) v over the cached keys j = 0 .. pos (pos = -1: none).
 
         q [B, H, head_dim]; rel [M, head_dim] of q's type with M >= max_len (the model's relative table) or None; key_pad uint8 / bool
-        [B, n], 1 = masked key.  A row without a key gives zeros.  nsplit: key ranges that run side by side (0: chosen from the sizes)."""
+        [B, n], 1 = masked key (a position tensor may pass n: keys from n on are not masked).  A row without a key gives zeros.  nsplit: key ranges that run side by side (0: chosen from the sizes)."""
         if key_pad is not None and key_pad.dtype is torch.bool:
             key_pad = key_pad.view(torch.uint8)
         key = (q.shape, q.stride(), q.dtype, q.device, rel is not None and (rel.shape, rel.stride(), rel.dtype, rel.device),

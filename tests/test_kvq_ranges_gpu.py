@@ -44,3 +44,23 @@ def test_queries_at_the_ends_of_the_range(T, q_at, k_at, dh, bits):
     for i, out in enumerate(outs):
         err = (out.cpu().double() - want).abs()
         assert bool((err <= bound).all()), (i, float(err.max()), float(bound.min()))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_sequences_whose_device_position_lies_outside_are_left_out(bits):
+    """as a whole, also where later rows of the call would reach into the cache; nothing of them is written, and they read as zeros"""
+    B, H, dh, n, room = 5, 2, 48, 70, 96
+    x = rows(B, n, H, dh, torch.bfloat16, 7)
+    p = torch.tensor([-1, -33, 96, -2 ** 31, 60], dtype=torch.int32, device="cuda")
+    d = x.cuda()
+    c = cache(B, H, room, dh, bits)
+    for t in (c.k, c.v):
+        t.fill_(0x21)
+    for t in (c.k_scale, c.v_scale):
+        t.fill_(3.0)
+    c.write(d[:, :, 1], d[:, :, 2], p)
+    for t, held in ((c.k, 0x21), (c.v, 0x21), (c.k_scale, 3.0), (c.v_scale, 3.0)):
+        assert bool((t[:4] == held).all()) and bool((t[4].flatten(1) != held).any())
+    for part, back in zip((1, 2), c.read(p, n, torch.bfloat16)):
+        assert bool((back[:4] == 0).all()) and bool((back[4, 36:] == 0).all())
+        assert same(back[4, :36].cpu(), expect_rows(x[4:, :36, part], bits, torch.bfloat16)[2][0])
