@@ -66,7 +66,7 @@ def generate(model, maps, device, out_dir, conditioning, short_filename=False,
     the device as one HIP graph per token while the KV cache is valid; False = one Python iteration per token) and
     `use_window_graph` (once the window slides, its full forward is replayed as one HIP graph per token).
     `min_p` > 0 drops tokens less likely than min_p times the most likely one (after top-k and the nucleus); `kv_bits` = 4 or 8 holds
-    the KV cache quantised.
+    the KV cache quantised (up to max_input_len tokens: behind that the window slides and every step is a full forward without a cache).
     `amp` is accepted for compatibility; the engine's precision is model.compute_dtype."""
     if not debug:
         os.makedirs(out_dir, exist_ok=True)
@@ -132,8 +132,8 @@ def generate(model, maps, device, out_dir, conditioning, short_filename=False,
         raise NotImplementedError("sampled generation supports vocabularies of at most %d symbols (got %d); use top_k=1 (greedy)" % (max_vocab, V))
     if not 0 <= min_p <= 1:
         raise ValueError("min_p must lie in [0, 1] (got %r)" % (min_p,))
-    if kv_bits and not use_cache:
-        raise ValueError("kv_bits quantises the KV cache: it needs use_cache")
+    if kv_bits and not (use_cache and varying_condition is None):
+        raise ValueError("kv_bits quantises the KV cache: it needs use_cache and no varying_condition (which recomputes every position)")
 
     cache_ok = bool(use_cache) and varying_condition is None
     sess = None
@@ -263,7 +263,7 @@ def main():
     parser.add_argument('--topk', type=int, default=-1)
     parser.add_argument('--topp', type=float, default=0.7)
     parser.add_argument('--minp', type=float, default=0.0, help="drop tokens less likely than this share of the most likely one (0: off)")
-    parser.add_argument('--kv_bits', type=int, default=None, choices=[4, 8], help="hold the KV cache in 4 or 8 bits (default: the model's own type)")
+    parser.add_argument('--kv_bits', type=int, default=None, choices=[4, 8], help="hold the KV cache in 4 or 8 bits (default: the model's own type); it serves the first max_input_len tokens, as without")
     parser.add_argument('--debug', action='store_true')
     parser.add_argument('--seed', type=int, default=0)
     parser.add_argument('--no_amp', action='store_true', help="run the exact-f32 tier instead of a 16-bit one")
