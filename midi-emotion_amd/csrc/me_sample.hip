@@ -52,7 +52,7 @@ struct SampleArgs {
     const int64_t* prev; const uint8_t* is_timeshift; float* repeats; const int32_t* pos;
     int pos0, u_ld; float temp_note, temp_rest, penalty;
     // wide rows: the workspace, the chunks
-    char* ws; int splits, chunk, B;
+    char* ws; int splits, chunk;
 };
 
 // workspace of a wide row (16-byte multiples); written before it is read by every call
@@ -871,7 +871,6 @@ int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st)
     }
     a.splits = splits_of(B, a.V);
     a.chunk = (a.V + a.splits - 1) / a.splits;
-    a.B = B;
     if (!ws || ((uintptr_t)ws & 15) || ws_bytes < (size_t)B * row_ws_bytes(a.splits)) return ME_ERR_WORKSPACE;
     a.ws = (char*)ws;
     static_assert(sizeof(Shared<WT>) + SL * 8 + 16 + ME_SAMPLE_MAX_VOCAB / 8 + 8 <= 65536, "a chunk of the widest row, with its barred ids");

@@ -383,7 +383,8 @@ _I64x6 = ctypes.c_int64 * 6
 
 
 def kvq_cache(kcodes, kscale, vcodes, vscale, dh, bits):
-    """host descriptor of a quantised cache (struct me_kvq_cache) for the calls below; the caller keeps the tensors"""
+    """host descriptor of a quantised cache (struct me_kvq_cache); the caller keeps the tensors.  me_kvq_write, me_kvq_read and me_kvq_attn are
+    called by kvcache.QuantKVCache, which checks what it hands them."""
     return ctypes.byref(_lib.KVQCache(_ptr(kcodes), _ptr(kscale), _ptr(vcodes), _ptr(vscale), kcodes.shape[0], kcodes.shape[1], int(dh), kcodes.shape[2], int(bits)))
 
 
@@ -392,40 +393,15 @@ def kvq_strides(k, v):
     return _I64x6(*k.stride()[:3], *v.stride()[:3])
 
 
-def kvq_write(cache, k, v, pos, lens=None, strides=None):
-    """quantise the rows k, v [B, n, H, dh] (any strides, dh contiguous) into the cache at positions pos .. (me_kvq_write)."""
-    t, t_dev, ld_t = _pos_args(pos)
-    check(lib().me_kvq_write(cache, _ptr(k), _ptr(v), strides or kvq_strides(k, v), k.shape[1], t, t_dev, ld_t, _ptr(lens), _code(k.dtype),
-                             _stream()), "me_kvq_write")
-
-
-def kvq_read(cache, k, v, pos, lens=None, strides=None):
-    """the rows at positions pos .. pos + n - 1 into k, v [B, n, H, dh] (me_kvq_read); rows from lens[b] on become zeros."""
-    t, t_dev, ld_t = _pos_args(pos)
-    check(lib().me_kvq_read(cache, _ptr(k), _ptr(v), strides or kvq_strides(k, v), k.shape[1], t, t_dev, ld_t, _ptr(lens), _code(k.dtype),
-                            _stream()), "me_kvq_read")
-
-
 def kvq_splits(B, H, tokens, rel=False):
     """key ranges me_kvq_attn should cut a cache of that many tokens into (1 .. 64)"""
     return int(lib().me_kvq_splits(int(B), int(H), int(tokens), int(bool(rel))))
 
 
-def kvq_attn(cache, q, out, pos, E=None, key_pad=None, part=None, nsplit=1):
-    """attention of one query per (sequence, head), q / out [B, H, dh], against the cached keys 0 .. pos (me_kvq_attn).
-    part: uninitialised f32 buffer of workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh) bytes where nsplit > 1; out = None
-    leaves the partial records in it (the form me_dec_proj_resid reads)."""
-    t, t_dev, ld_t = _pos_args(pos)
-    qb, qh, _ = q.stride()
-    ob, oh, _ = out.stride() if out is not None else (0, 0, 0)
-    check(lib().me_kvq_attn(cache, _ptr(q), qb, qh, _ptr(E), E.shape[0] if E is not None else 0, _ptr(key_pad),
-                            key_pad.shape[1] if key_pad is not None else 0, _ptr(out), ob, oh, _ptr(part),
-                            part.numel() * part.element_size() if part is not None else 0, nsplit, t, t_dev, ld_t, _code(q.dtype), _stream()),
-          "me_kvq_attn")
-
-
 def kvq_append_attn(cache, q, k, v, out, pos, E=None, key_pad=None, part=None, nsplit=1):
-    """kvq_write of the rows k, v [B, H, dh] (equal strides) at pos and kvq_attn over the keys 0 .. pos in one launch (me_kvq_append_attn)."""
+    """the rows k, v [B, H, dh] (equal strides) written at pos and the attention of q over the keys 0 .. pos in one launch (me_kvq_append_attn).
+    part: uninitialised f32 buffer of workspace_bytes(ME_WS_KVQ_ATTN, B * H, nsplit, dh) bytes where nsplit > 1; out = None leaves the partial
+    records in it (the form me_dec_proj_resid reads)."""
     t, t_dev, ld_t = _pos_args(pos)
     qb, qh, _ = q.stride()
     nb, nh, _ = k.stride()
