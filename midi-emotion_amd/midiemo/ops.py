@@ -441,6 +441,9 @@ def _sample_rows(B, V, logits, special, rows, ids, n_choices):
     shape, stride = logits.shape, logits.stride()
     if not (logits.dtype is f32 and len(shape) == 2 and shape[0] == B and shape[1] >= V and stride[1] == 1):
         raise RuntimeError("sampling: logits must be float32 [%d, >= %d] with contiguous rows (got %s %s)" % (B, V, logits.dtype, tuple(shape)))
+    ld = stride[0] if B > 1 else V                            # a C int: ctypes would cut a larger one to 32 bits
+    if ld >= 1 << 31:
+        raise RuntimeError("sampling: rows of logits must lie less than 2^31 elements apart (got %d)" % ld)
     for x in rows:
         if not (x.dtype is f32 and x.numel() == B and x.is_contiguous() and x.get_device() == dev):
             raise RuntimeError("sampling: one contiguous float32 value per sequence is needed on %s (got %s %s on %s)" % (logits.device, x.dtype, tuple(x.shape), x.device))
@@ -453,7 +456,7 @@ def _sample_rows(B, V, logits, special, rows, ids, n_choices):
     lg = _ptr(logits)
     if dev != torch.cuda.current_device():
         raise RuntimeError("sampling: the tensors are on %s, the current device is %d" % (logits.device, torch.cuda.current_device()))
-    return (torch._C._cuda_getCurrentRawStream(dev), lg, stride[0], V, special.data_ptr() if special is not None else None, special.numel() if special is not None else 0,
+    return (torch._C._cuda_getCurrentRawStream(dev), lg, ld, V, special.data_ptr() if special is not None else None, special.numel() if special is not None else 0,
             [x.data_ptr() for x in rows], [x.data_ptr() for x in ids], n_choices.data_ptr() if n_choices is not None else None)
 
 
@@ -471,8 +474,9 @@ def sample_minp_step(logits, V, special, prev_tok, is_timeshift, repeat_counts, 
     """sample_step with min-p and for wide vocabularies (me_sample_minp_step)"""
     B = out_ids.numel()
     if not (is_timeshift.dtype is torch.uint8 and is_timeshift.numel() >= V and is_timeshift.is_contiguous() and u_table.dtype is torch.float32 and
-            u_table.dim() == 2 and u_table.size(1) >= B and u_table.stride(1) == 1 and pos.dtype is torch.int32):
-        raise RuntimeError("sampling: a step needs uint8 time-shift marks [>= %d], float32 uniforms [steps, >= %d] and an int32 position" % (V, B))
+            u_table.dim() == 2 and u_table.size(1) >= B and u_table.stride(1) == 1 and pos.dtype is torch.int32 and
+            is_timeshift.get_device() == u_table.get_device() == pos.get_device() == logits.get_device()):
+        raise RuntimeError("sampling: a step needs uint8 time-shift marks [>= %d], float32 uniforms [steps, >= %d] and an int32 position, all on %s" % (V, B, logits.device))
     stream, lg, ld, V, sp, n_sp, (rc,), (prev, out), nc = _sample_rows(B, V, logits, special, (repeat_counts,), (prev_tok, out_ids), n_choices)
     ws = _sample_ws(B, V, logits.device) if V > _lib.ME_SAMPLE_ONE_BLOCK else None
     check(lib().me_sample_minp_step(lg, ld, V, sp, n_sp, prev, _ptr(is_timeshift), rc, float(temp_note), float(temp_rest), float(penalty_coeff),
