@@ -176,14 +176,9 @@ def tier_parity_sample():
 
 
 def source_hash():
-    """sha256 over the kernel sources: ties profiles/hbm_traffic.json (a PMC pass) to the code it was measured on."""
-    import hashlib
-    h = hashlib.sha256()
-    cs = os.path.join(ROOT, "midi-emotion_amd", "csrc")
-    for n in sorted(os.listdir(cs)):
-        if n.endswith((".hip", ".h")):
-            h.update(open(os.path.join(cs, n), "rb").read())
-    return h.hexdigest()
+    """sha256 over the kernel sources of the train step: ties profiles/hbm_traffic.json (a PMC pass) to the code it was measured on."""
+    from midiemo.build import step_source_hash
+    return step_source_hash(os.path.join(ROOT, "midi-emotion_amd", "csrc"))
 
 
 def decode_bytes(c, t, B, elt=2):

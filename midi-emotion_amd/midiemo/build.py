@@ -1,5 +1,6 @@
 """Builds libmidiemo_hip.so (gfx950 only) in-tree with hipcc.  No torch headers,
 no hipify, no multi-arch: the library is a plain C-ABI shared object."""
+import hashlib
 import os
 import shutil
 import subprocess
@@ -22,6 +23,19 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=f
 # (test_dec_ln_proj and test_resid_ln_fwd_bwd in f16, each by one rounding step).
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FIXED_ROUNDING = ("me_gemm.hip", "me_elem.hip", "me_attn.hip", "me_attn64.hip", "me_decode.hip", "me_decode_token.hip")
+
+
+# what the train step's kernels are built from: a profile of the step stands as long as these files do
+STEP_SOURCES = ("me_attn.hip", "me_attn64.hip", "me_attn_common.h", "me_common.h", "me_elem.hip", "me_gemm.hip")
+
+
+def step_source_hash(csrc=CSRC):
+    """sha256 over the kernel sources of the train step: ties the committed profiles of the step to the code they were measured on."""
+    h = hashlib.sha256()
+    for n in STEP_SOURCES:
+        with open(os.path.join(csrc, n), "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
 
 
 def _hipcc():

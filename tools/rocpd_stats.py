@@ -43,7 +43,7 @@ def main():
         print("%-62s %7d %12.1f %10.2f %10.2f %10.2f %6.2f" % (k[:62], a[0], a[1] / 1e3, a[1] / a[0] / 1e3, a[2] / 1e3, a[3] / 1e3, 100 * a[1] / tot))
     print("total kernel time: %.3f ms" % (tot / 1e6) + (", per step %.3f ms" % (tot / 1e6 / steps) if steps else ""))
     if jpath and steps:
-        import hashlib, json, os
+        import json, os
         fam = {}
         for n, d in rows:
             for f, keys in FAMILIES:
@@ -51,14 +51,11 @@ def main():
                     a = fam.setdefault(f, [0, 0.0])
                     a[0] += 1; a[1] += d
                     break
-        cs = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "midi-emotion_amd", "csrc")
-        h = hashlib.sha256()
-        for n_ in sorted(os.listdir(cs)):
-            if n_.endswith((".hip", ".h")):
-                h.update(open(os.path.join(cs, n_), "rb").read())
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "midi-emotion_amd"))
+        from midiemo.build import step_source_hash
         out = {"families": {f: {"launches_per_step": round(a[0] / steps, 2), "avg_us": round(a[1] / a[0] / 1e3, 2),
                                 "ms_per_step": round(a[1] / 1e6 / steps, 4)} for f, a in fam.items()},
-               "steps": steps, "kernel_ms_per_step": round(tot / 1e6 / steps, 4), "_source_sha256": h.hexdigest(),
+               "steps": steps, "kernel_ms_per_step": round(tot / 1e6 / steps, 4), "_source_sha256": step_source_hash(),
                "_profile": os.environ.get("PROFILE_TAG", "profiles/")}
         json.dump(out, open(jpath, "w"), indent=1)
 
