@@ -147,7 +147,7 @@ template <int BITS, bool WIDE> ME_DEV void quantise8(const float (&x)[8], u16& s
 // ---------------------------------------------------------------------------------------------------------
 // write: block = one 32-token block of one (sequence, head): 8 lanes per row, so that a row's maximum takes three lane
 // exchanges and its 16-bit values one 16-byte load per lane.  Bounded by memory where there is enough of it: 32 x 2048 x 8 rows of 64 in
-// bf16, 4 bits: 33.5 us = 5.1 TB/s of K, V, codes and scales moved (a copy reaches 5.0); 64 x 8 rows (a step): 3.7 us, a launch's latency.  K goes straight to its chunk (4 / 8 bytes per
+// bf16, 4 bits: 33.8 us = 5.0 TB/s of K, V, codes and scales moved (a copy reaches 5.0); 64 x 8 rows (a step): 3.7 us, a launch's latency.  K goes straight to its chunk (4 / 8 bytes per
 // lane); V changes its order through LDS (8 tokens of a dimension per thread), and a group of 8 tokens that the call covers only in
 // part keeps its other codes (read, merged, written by the one thread that owns the word).
 // ---------------------------------------------------------------------------------------------------------
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void kvq_write_kernel(const RowArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// read back: the same split (27.1 us = 6.3 TB/s for the rows above: mostly stores); a row behind the sequence's length (or the cache's end) reads as zeros
+// read back: the same split (27.3 us = 6.2 TB/s for the rows above: mostly stores); a row behind the sequence's length (or the cache's end) reads as zeros
 // ---------------------------------------------------------------------------------------------------------
 template <int BITS> ME_DEV void expand8(float (&x)[8], uint32_t c0, uint32_t c1, float s) {
     f32x2_t r[4];
@@ -300,9 +300,10 @@ __global__ __launch_bounds__(256) void kvq_read_kernel(const RowArgs a) {
 //      the chunk that belongs to the row's 16 keys); V: the weights p_j * scale_j (4 bits: scaled by a power of two per tile) are the rows.
 //   E is shared by a block's heads: its products for a stretch of keys come from one matrix product per 16 keys and wait in LDS.
 // What bounds it: long caches the memory, 64 x 8 heads x 16384 keys of 64 in 4 bits 97 us = 5.9 TB/s; with the relative products and a
-// mask, 64 x 16 x 1999 of 48 in 8 bits, 37.7 us = 5.4 TB/s; few rows the chain of latencies: 1 x 8 x 256: 5.5 us, 4 x 8 x 2048: 8.0 us with its
-// join, where 4.5 MB would take 0.9.  A tile of 128 keys is two K operands' columns of 64 lanes (a lane holds two logits) and one V operand's
-// depth, and the next tile's loads are in flight under a tile's products.
+// mask, 64 x 16 x 1999 of 48 in 8 bits (ragged), 42 us = 4.3 TB/s; with them alone, 64 x 8 x 2048 of 64 in 4 bits, 23 us = 3.1 TB/s: a block's
+// products precede its stream.  Few rows: the chain of latencies, 1 x 8 x 256: 5.7 us, 4 x 8 x 2048: 8.3 us with its join, where 4.5 MB would
+// take 0.9.  With the step's rows written too 0.9 .. 1.6 us more (64 x 16 x 1999: 2.9); without the join, as a decode step calls it, 6.1 and 7.6.
+// A tile of 128 keys is two K operands' columns of 64 lanes (a lane holds two logits) and one V operand's depth, and the next tile's loads are in flight under a tile's products.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int RELS = 4096;                                    // relative logits in LDS: a stretch of RELS / (heads of the block) keys
 constexpr int TK = 128;                                       // keys per tile
@@ -917,7 +918,7 @@ int me_kvq_read(const me_kvq_cache* c, void* k, void* v, const int64_t* strides,
 // How the keys are cut.  2048 waves (8 per CU) are enough to keep the memory busy; a row (sequence, head) that has fewer is cut into
 // ranges: first inside the block (ranges meet in LDS), then over blocks, whose records a second launch joins (2 .. 3 us).  The
 // relative products want blocks of many heads (a stretch's rows of E are read once per block) but 256 blocks, one per CU, come first.
-// Measured, us per call, 4 bits, dh 64, one block per row and all ranges in it -> as chosen here:
+// Measured, us per call of one cache replayed (it stays in the last-level cache), 4 bits, dh 64, one block per row and all ranges in it -> as chosen here:
 //   relative table: 1 x 8 rows of 2048 keys 13.5 -> 7.4, 4 x 8: 14.5 -> 8.0, 16 x 8: 15.6 -> 11.2, 64 x 8: 34.0 -> 20.4; up to 512 keys
 //   one launch is faster (4 x 8 of 512: 6.5, four splits 7.0);  none: 1 x 8 of 16384 keys 8 splits 9.2, 16: 8.5; 16 x 8 of 4096: two splits 12.6, none 12.0.
 int me_kvq_splits(int B, int H, int tokens, int rel) {

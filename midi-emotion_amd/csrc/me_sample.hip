@@ -15,10 +15,12 @@
 // row, bins and lists in its LDS.  Wider ones take four launches: the chunks' maxima; the chunks' histograms; the members of
 // the bins that can hold one of the borders (known up to a bin or two from the histogram alone), gathered by all chunks; and one block per
 // row that finishes on those few entries.  Measured, us a call in a graph, top_p 0.9 and min_p 0.05 / top_k 200, top_p 0.95 and min_p 0.02:
-//   one block, 256 threads:   4 x 1018: 7.6 / 12.7,  64 x 2048: 10.5 / 14.5,  512 x 1018: 10.4 / 14.1
-//   one block, 1024 threads:  64 x 32000: 23.7 / 24.2 (0.34 TB/s: 64 of 256 CUs),  256 x 32512: 29.6 / 28.3 (1.2 TB/s)
-//   four launches:            1 x 131071: 27.7 / 32.4,  128 x 131071: 64.7 / 76.9 (1.0 TB/s; the row is read three times, from the
-//                             last-level cache: maxima 12, histograms 28, gathering 20, finish 15 us)
+//   one block, 256 threads:   4 x 1018: 7.7 / 11.1,  64 x 2048: 10.5 / 14.4,  512 x 1018: 10.5 / 14.4
+//   one block, 1024 threads:  64 x 32000: 23.6 / 24.2 (0.35 TB/s: 64 of 256 CUs),  256 x 32512: 27.8 / 28.1 (1.2 TB/s)
+//   four launches:            1 x 131071: 27.8 / 32.4,  128 x 131071: 64.8 / 77.0 (1.0 TB/s; the row is read three times, from the
+//                             last-level cache: maxima 12, histograms 29, gathering 21, finish 15 us)
+// Rows whose logits lie close together put more than 4096 entries into a border's bin; the last launch then walks the row itself, one block for
+// each, twice for every level of a search: 128 x 131071 of equal logits 1065 / 1524 us, of deviation 0.1 (temperature 1) 1173 / 93; 64 x 32000: 213 / 288, 113 / 41.
 #include "me_common.h"
 #include <algorithm>
 #include <math.h>
@@ -35,8 +37,8 @@ constexpr int NL = 128;                     // entries that are compared with ea
 constexpr int GL = 4096;                    // gathered entries of a wide row
 constexpr int FRAC = 45;                    // weight unit 2^-45
 // 32512: the row, the bins and the lists fill 160 KB of LDS.  Up to there one block is faster at every batch measured, although
-// few rows leave CUs idle: 32512 symbols in one block / 32513 in four launches, us: 1 row 22.3 / 25.3, 8: 22.8 / 28.4, 64: 23.4 / 38.6, 512: 53.2 / 66.1
-// (top_p 0.9, min_p 0.05; where a border falls into a full bin both take longer, and for a single row it was 31.3 / 25.9)
+// few rows leave CUs idle: 32512 symbols in one block / 32513 in four launches, us: 1 row 22.4 / 25.5, 8: 23.0 / 28.3, 64: 25.0 / 38.4, 512: 52.9 / 67.2
+// (top_p 0.9, min_p 0.05; nearest to each other for a single row with top_p 0.98, min_p 0.001: 25.6 / 26.2)
 constexpr int ONE_BLOCK = ME_SAMPLE_ONE_BLOCK;
 constexpr int MAX_SPLIT = 16;               // chunks of a wide row at most: every later block reads all chunks' histograms
 
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a) {
 
 // ---------------------------------------------------------------------------------------------------------
 // wider rows: grid (splits, B) blocks of a chunk each.  Bounded by the histogram's and the gathering's instructions, about 30 an entry
-// (128 x 131071: 28 and 20 us; their bytes alone would take 13 us each at the rate of a copy)
+// (128 x 131071: 29 and 21 us; their bytes alone would take 13 us each at the rate of a copy)
 // ---------------------------------------------------------------------------------------------------------
 constexpr int WT = 512;                                       // threads of a chunk's block
 constexpr int PT = 256;                                       // and of the block that finishes a row
@@ -859,7 +861,7 @@ double least_exponent(float min_p) { return log2((double)min_p) - 0x1p-54 * 1.44
 int sample_call(SampleArgs& a, int B, void* ws, size_t ws_bytes, hipStream_t st) {
     static bool big1[64] = {}, big2[64] = {};
     if (a.V <= ONE_BLOCK) {
-        // 256 threads to 2048 symbols: fewer waves meet at each barrier (2048 symbols on 256 / 2049 on 1024 threads: 4 rows 8.4 / 10.5 us, 64: 10.5 / 12.7)
+        // 256 threads to 2048 symbols: fewer waves meet at each barrier (2048 symbols on 256 / 2049 on 1024 threads: 4 rows 8.6 / 10.6 us, 64: 10.5 / 11.2)
         if (a.V <= 2048) sample_row_kernel<256><<<B, 256, sizeof(Shared<256>) + SL * 8 + (size_t)(a.V + 3) / 4 * 16, st>>>(a);
         else {
             static_assert(sizeof(Shared<1024>) + SL * 8 + (size_t)ONE_BLOCK * 4 <= 160 * 1024, "the widest row of one block");
