@@ -99,10 +99,12 @@ class QuantKVCache:
         return k.shape[1], ops.kvq_strides(k, v), ops._code(k.dtype)
 
     def _check_new(self, q, k, v):
+        # a dimension of one entry has no stride of its own: torch leaves any number there, also in what it calls contiguous
+        step = lambda x: tuple(d if n == 1 else s for s, n, d in zip(x.stride(), x.shape, (self.heads * self.head_dim, self.head_dim, 1)))
         for x in (k, v):
-            _need(x.shape == (self.batch, self.heads, self.head_dim) and x.dtype == q.dtype and x.stride() == k.stride() and x.stride(2) == 1,
+            _need(x.shape == (self.batch, self.heads, self.head_dim) and x.dtype == q.dtype and step(x) == step(k) and x.stride(2) == 1,
                   "new rows must be [%d, %d, %d] of q's type with equal strides and the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(x.shape)))
-        return k.stride()[:2]
+        return step(k)[:2]
 
     def _check_attend(self, q, rel, key_pad, out):
         _need(q.dim() == 3 and q.shape == (self.batch, self.heads, self.head_dim) and q.stride(2) == 1, "q must be [%d, %d, %d] with the last dimension contiguous, got %s" % (self.batch, self.heads, self.head_dim, tuple(q.shape)))
