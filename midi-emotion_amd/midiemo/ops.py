@@ -439,7 +439,7 @@ def _sample_rows(B, V, logits, special, rows, ids, n_choices):
     """The current stream and the address of each of a sampling call's tensors, all looked at first: rows = the f32 values, ids = the int64 ones, one per sequence."""
     dev, f32 = logits.get_device(), torch.float32
     shape, stride = logits.shape, logits.stride()
-    if not (logits.dtype is f32 and len(shape) == 2 and shape[0] == B and shape[1] >= V and stride[1] == 1):
+    if not (logits.dtype is f32 and len(shape) == 2 and shape[0] == B and shape[1] >= V and (stride[1] == 1 or shape[1] == 1)):
         raise RuntimeError("sampling: logits must be float32 [%d, >= %d] with contiguous rows (got %s %s)" % (B, V, logits.dtype, tuple(shape)))
     ld = stride[0] if B > 1 else V                            # a C int: ctypes would cut a larger one to 32 bits
     if ld >= 1 << 31:
@@ -474,7 +474,7 @@ def sample_minp_step(logits, V, special, prev_tok, is_timeshift, repeat_counts, 
     """sample_step with min-p and for wide vocabularies (me_sample_minp_step)"""
     B = out_ids.numel()
     if not (is_timeshift.dtype is torch.uint8 and is_timeshift.numel() >= V and is_timeshift.is_contiguous() and u_table.dtype is torch.float32 and
-            u_table.dim() == 2 and u_table.size(1) >= B and u_table.stride(1) == 1 and pos.dtype is torch.int32 and
+            u_table.dim() == 2 and u_table.size(1) >= B and (u_table.stride(1) == 1 or u_table.size(1) == 1) and pos.dtype is torch.int32 and
             is_timeshift.get_device() == u_table.get_device() == pos.get_device() == logits.get_device()):
         raise RuntimeError("sampling: a step needs uint8 time-shift marks [>= %d], float32 uniforms [steps, >= %d] and an int32 position, all on %s" % (V, B, logits.device))
     stream, lg, ld, V, sp, n_sp, (rc,), (prev, out), nc = _sample_rows(B, V, logits, special, (repeat_counts,), (prev_tok, out_ids), n_choices)
